@@ -13,7 +13,10 @@ SOURCES = ["gemm.hip", "attention.hip", "layernorm.hip", "tokens.hip", "loss.hip
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wall", "-Wno-unused-function",
          # keep MFMA accumulators in arch VGPRs: with the default AGPR form hipcc (ROCm 7.2) copied every accumulator in
          # and out of the AGPR file each loop iteration (100 v_accvgpr_* per 16 MFMAs in the GEMM main loop)
-         "-mllvm", "-amdgpu-mfma-vgpr-form"]
+         "-mllvm", "-amdgpu-mfma-vgpr-form",
+         # no packed f32 arithmetic (v_pk_add / mul / fma_f32): some of its forms gave wrong results on these machines now and then, and a
+         # packed f32 op issues in two passes anyway
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 # attention.hip: no SLP vectorisation.  hipcc packs neighbouring f32 multiplies of MFMA accumulator registers into v_pk_mul_f32
@@ -31,7 +34,7 @@ def _stale(target, deps):
 
 
 def build(force=False, verbose=False):
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm8.h"), os.path.join(CSRC, "gemm_k2.h"), os.path.join(CSRC, "gemm_r3.h"), os.path.join(CSRC, "gemm_r4.h"), os.path.join(HERE, "..", "include", "mofo_hip.h"), os.path.abspath(__file__)]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "attn_tile.h"), os.path.join(CSRC, "gemm8.h"), os.path.join(CSRC, "gemm_k2.h"), os.path.join(CSRC, "gemm_r3.h"), os.path.join(CSRC, "gemm_r4.h"), os.path.join(HERE, "..", "include", "mofo_hip.h"), os.path.abspath(__file__)]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
     jobs = []

@@ -75,8 +75,8 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// erf-form GELU and its derivative (nn.GELU() default, modeling_finetune.py:35), two elements at a time in packed fp32
-// (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth of FMA per issue slot).  The Gaussian cdf is an odd minimax polynomial
+// erf-form GELU and its derivative (nn.GELU() default, modeling_finetune.py:35), two elements at a time
+// (two independent chains; the build turns packed f32 instructions off).  The Gaussian cdf is an odd minimax polynomial
 // 0.5 + x * P(x^2) on |x| <= 4 (degree 8 in x^2, |error| <= 4e-6 inside the clamp, <= 3.2e-5 = 1 - cdf(4) beyond it --
 // two orders below the bf16 rounding of the stored result); no transcendental and no division, where the previous
 // Abramowitz-Stegun form spent a v_exp + v_rcp (quarter rate each) per element and made the K=384 GELU epilogues

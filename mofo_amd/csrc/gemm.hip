@@ -143,7 +143,7 @@ __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned 
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                      :
                      : "s"((unsigned)(unsigned long long)LDS_PTR(lds_dst)), "v"(voff), "s"(rsrc), "s"(soff)
-                     : "memory");
+                     : "memory", "vcc");   // no operand in vcc: a VALU compare next to the piece may write it inside the hazard window
     } else {
         unsigned keep;
         asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
