@@ -187,6 +187,41 @@ int mofo_attention_bwd_dkv_range(const void* qkv, int ldqkv, const void* dout, i
 int mofo_attention_bwd_dq_delta_range(const void* qkv, int ldqkv, const void* out, int ldo, const void* dout, int lddo, const float* lse2,
                                       float* delta_out, int B, int N, int H, float scale, int q_begin, void* dqkv, int lddqkv, void* stream);
 
+/* ---- rotary positions over several axes (time, row, column of the token grid), forward and gradient (inverse != 0: the same turn by
+ * the negative angle).  x, out [M, heads * head_dim], f32 or bf16 (x_is_bf16), row pitches ldx / ldo; out may be x (in place).  The first
+ * 2 * pairs columns of every head turn, pairs = the sum of sections[0 .. naxes) (host array, up to 4 axes); the others are copied.
+ * Pair i is columns (i, pairs + i) of the head, or (2 i, 2 i + 1) when interleaved; axis a owns sections[a] consecutive pairs.
+ * freqs f64 [pairs]: TURNS per position (angle / 2 pi).  Places: pos i32 [M, naxes], or tok_idx i32 [M] = token ids >= 0 on a grid of
+ * rows grid_h x grid_w (id = (t * grid_h + h) * grid_w + w, what mofo_mask_to_indices writes); exactly one of the two.
+ * pairs a multiple of 8 up to 128, head_dim a multiple of 16 up to 1024; rows in 16-byte aligned pieces. ---- */
+int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, int ldo, int M, int heads, int head_dim, const double* freqs, int naxes,
+                   const int* sections, const int* pos, const int* tok_idx, int grid_h, int grid_w, int interleaved, int inverse, void* stream);
+
+/* ---- differential attention: two softmax maps a head, their difference with a learned weight.  For head h (H of them, key head h / (H / Hkv)):
+ *   S_m = scale * q_m k_m^T,  P_m = softmax(S_m) over the row's visible keys (m = 1, 2; 64 columns each)
+ *   lam = exp(l0 . l1) - exp(l2 . l3) + lam_init,   o2 = P_2 v,   o = P_1 v - lam o2     (v, o, o2: 128 columns)
+ *   out = gamma ? out_scale * gamma * o / sqrt(mean(o^2) + eps) : o
+ * q bf16 [B * Nq, H * 128] (q_1 | q_2 per head), k, v bf16 [B * Nk, Hkv * 128]: column ranges of one packed projection, or a cache of Nk rows
+ * a clip.  lam [4][lam_heads][64] (lam_heads 1 = shared, or H), gamma [128] or NULL; both f32, or bf16 when param_is_bf16.
+ * Key j of clip b is visible to query i iff j < kv_len[b] (i32 [B]; NULL: Nk; values are cut to 0 .. Nk) and, causal = 1: j <= i;
+ * causal = 2: j <= i + kv_len[b] - Nq (new tokens at the end of a cache).  A row that sees nothing gives zeros, and takes none of
+ * the gradients.  Rows of k, v at and behind kv_len[b] may hold anything; rows in front of it are expected to be finite.
+ * For the gradient keep o, o2 (bf16 [B * Nq, H * 128], contiguous) and lse2 (f32 [2, B, H, Nq], log2-sum-exp2); NULL all three otherwise.
+ * ws: mofo_diff_attention_fwd_ws floats of scratch (0: NULL is fine), contents of no interest; two calls that may run at once (two
+ * streams, two captured graphs) need one each. ---- */
+long long mofo_diff_attention_fwd_ws(int B, int Nq, int Nk, int H, int Hkv);
+int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
+                            const void* lam, int lam_heads, float lam_init, const void* gamma, int param_is_bf16, float eps, float out_scale,
+                            const int* kv_len, int causal, void* out, int ldo, void* o, void* o2, float* lse2, float* ws, long long ws_elems, void* stream);
+/* Every gradient of it, overwritten: dq like q, dk and dv like k and v (summed over the heads that share them; zero at and behind kv_len),
+ * dlam like lam, dgamma like gamma (both f32, or bf16 when grad_is_bf16).  norm: whether gamma is given.  Plain stores and fixed orders
+ * only: the same inputs give the same bits. */
+long long mofo_diff_attention_bwd_ws(int B, int Nq, int Nk, int H, int Hkv, int norm);
+int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
+                            const void* lam, int lam_heads, float lam_init, const void* gamma, int param_is_bf16, float eps, float out_scale,
+                            const int* kv_len, int causal, const void* o, const void* o2, const float* lse2, const void* dout, int lddo, void* dq, int lddq,
+                            void* dk, int lddk, void* dv, int lddv, void* dlam, void* dgamma, int grad_is_bf16, float* ws, long long ws_elems, void* stream);
+
 /* ---- RCCL communicator: the stand-alone route to the ONE collective of the path -- the per-step gradient
  * all-reduce of run_mae_pretraining.py:225-227 (DDP) over the group of utils.py:289-294 -- for callers that bind this library
  * without torch.distributed (mofo_amd/dist.py itself uses torch.distributed's "nccl" = RCCL backend).  librccl is opened at

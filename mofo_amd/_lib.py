@@ -61,6 +61,12 @@ _SIGS = {
     "mofo_attention_bwd_dq_range": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _f, _i, _vp, _i, _vp]),
     "mofo_attention_bwd_dq_delta_range": (_i, [_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _f, _i, _vp, _i, _vp]),
     "mofo_attention_bwd_dkv_range": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _f, _i, _vp, _i, _vp]),
+    "mofo_rope_axes": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "mofo_diff_attention_fwd_ws": (_ll, [_i, _i, _i, _i, _i]),
+    "mofo_diff_attention_fwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _f, _vp, _i, _f, _f, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _ll, _vp]),
+    "mofo_diff_attention_bwd_ws": (_ll, [_i, _i, _i, _i, _i, _i]),
+    "mofo_diff_attention_bwd": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _f, _vp, _i, _f, _f, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i,
+                                     _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _ll, _vp]),
     "mofo_mask_to_indices": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "mofo_tube_masks": (_i, [C.c_uint, C.c_uint, _i, _i, _i, _i, _vp, _vp]),
     "mofo_patch_gather": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp]),

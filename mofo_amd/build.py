@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmofo_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-SOURCES = ["gemm.hip", "attention.hip", "layernorm.hip", "tokens.hip", "loss.hip", "optim.hip", "quant.hip", "capi.cpp", "comm.cpp"]
+SOURCES = ["gemm.hip", "attention.hip", "diff_attention.hip", "rope.hip", "layernorm.hip", "tokens.hip", "loss.hip", "optim.hip", "quant.hip", "capi.cpp", "comm.cpp"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wall", "-Wno-unused-function",
          # keep MFMA accumulators in arch VGPRs: with the default AGPR form hipcc (ROCm 7.2) copied every accumulator in
          # and out of the AGPR file each loop iteration (100 v_accvgpr_* per 16 MFMAs in the GEMM main loop)
@@ -23,7 +23,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=f
 # plus v_mov shuffles; a packed f32 op issues in two passes anyway (guide MI355X_MICROARCH.md: an anti-lever beside MFMAs), and
 # these kernels are bound by the SIMD's vector issue port.  (Inline-asm single multiplies are not an option: an asm VALU that
 # reads an MFMA result gets none of the compiler's hazard wait states -- it read stale accumulators.)
-EXTRA_FLAGS = {"attention.hip": ["-fno-slp-vectorize"]}
+EXTRA_FLAGS = {"attention.hip": ["-fno-slp-vectorize"], "diff_attention.hip": ["-fno-slp-vectorize"]}
 
 
 def _stale(target, deps):

@@ -1,6 +1,5 @@
 // Tile helpers of the attention kernels (attention.hip, diff_attention.hip): LDS image of a [32 rows][64 columns] bf16 tile, its MFMA
 // operand fragments in both directions, LDS-DMA pieces, XCD-aware block decode.  Included inside each file's anonymous namespace.
-#pragma once
 
 // raised priority while a wave issues its MFMA groups: the matrix pipe is fed first, other waves' VALU fills the issue gaps
 #define ATTN_PRIO(x) __builtin_amdgcn_s_setprio(x)

@@ -1,0 +1,734 @@
+// Differential attention for gfx950, bf16 in / f32 accumulate, forward and gradient.
+//
+// A head has TWO softmax maps over 64-wide queries / keys and one 128-wide value (a head row is q1|q2, k1|k2, v: 128 columns each):
+//     S_m = scale * Q_m K_m^T,   P_m = softmax over the row's visible keys,   lam = exp(l0.l1) - exp(l2.l3) + lam_init,
+//     O = (P1 - lam P2) V,       Y = out_scale * gamma * O / sqrt(mean(O^2) + eps)      (Y = O without gamma).
+// Query rows of the G = H / Hkv heads that share a key head are ONE list of R = G * Nq rows (row g * Nq + i): shared key heads cost
+// nothing extra in any pass and their gradients are summed inside a block, in a fixed order.
+// Every mask here is a prefix: row i of clip b sees keys j < lim(b, i), lim = kv_len[b], cut at i + 1 (causal from the start) or at
+// kv_len[b] - Nq + i + 1 (causal towards the end, new tokens behind a cache).  lim = 0: the row's outputs and gradients are zero.
+// Rows of k / v at and behind kv_len[b] are never used: they are replaced by zeros on the way into LDS, whatever they hold.
+//
+// As in attention.hip, the first product is formed with the "other" sequence index on the LANE (v_mfma_f32_32x32x16_bf16):
+//   forward / dQ : S^T[key][row] = K . Q^T, row softmax in-lane + one half swap;      dK, dV : S[row][key] = Q . K^T
+// so the accumulator, packed to bf16, is the B operand of the second product.  Rounding to bf16 of P and dS is the only rounding
+// between the inputs and the f32 accumulators; softmax sums, statistics and norms stay f32.
+#include "common.h"
+#include "../../include/mofo_hip.h"
+#include <type_traits>
+
+namespace {
+
+#include "attn_tile.h"
+
+constexpr int HV = 128;                 // columns of a head's q, k, v and output rows
+constexpr float EMPTY_LSE = 1.0e30f;    // log-sum of a row that sees nothing: exp2(s - 1e30) = 0
+constexpr float BIG_LOG2 = 20.f;        // forward: a row's reference maximum is kept until a tile's partial sum passes 2^20
+
+struct DiffArgs {
+    const bf16_t *q, *k, *v;
+    size_t ldq, ldk, ldv;
+    int B, H, Hkv, G, Nq, Nk, R, causal;
+    const int* kv_len;
+    const void* lam;          // [4][lam_heads][64]
+    const void* gamma;        // [128] or NULL
+    int param_bf16, lam_heads;
+    float lam_init, scale, c, eps, out_scale;
+};
+
+__device__ __forceinline__ int clip_len(const DiffArgs& a, int b) {
+    if (!a.kv_len) return a.Nk;
+    const int n = a.kv_len[b];
+    return n < 0 ? 0 : n > a.Nk ? a.Nk : n;
+}
+__device__ __forceinline__ int row_lim(const DiffArgs& a, int len, int i) {
+    if (a.causal == 0) return len;
+    const int last = (a.causal == 1 ? i : len - a.Nq + i) + 1;
+    return last < 0 ? 0 : last < len ? last : len;
+}
+// smallest and largest limit of the rows ra .. rb (inclusive) of the list: monotone within a head
+__device__ __forceinline__ void span_lim(const DiffArgs& a, int len, int ra, int rb, int& lo, int& hi) {
+    if (a.causal == 0) {
+        lo = hi = len;
+        return;
+    }
+    const bool one = a.G == 1 || ra / a.Nq == rb / a.Nq;
+    lo = row_lim(a, len, one ? ra % a.Nq : 0);
+    hi = row_lim(a, len, one ? rb % a.Nq : a.Nq - 1);
+}
+__device__ __forceinline__ float param(const void* p, int bf, size_t i) { return bf ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i]; }
+// lambda of head h, and its two exponentials (every lane of the wave)
+__device__ __forceinline__ float head_lambda(const DiffArgs& a, int h, int lane, float& e1, float& e2) {
+    const int hl = a.lam_heads == 1 ? 0 : h;
+    const size_t st = (size_t)a.lam_heads * 64, o = (size_t)hl * 64 + lane;
+    e1 = expf(wave_sum(param(a.lam, a.param_bf16, o) * param(a.lam, a.param_bf16, st + o)));
+    e2 = expf(wave_sum(param(a.lam, a.param_bf16, 2 * st + o) * param(a.lam, a.param_bf16, 3 * st + o)));
+    return e1 - e2 + a.lam_init;
+}
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
+
+// one lane's row of a wave tile
+struct Row {
+    bool valid;
+    int r, h, i, lim;
+    size_t at;      // row of q / out / dout: b * Nq + i
+    size_t st;      // index into the [B, H, Nq] statistics
+};
+__device__ __forceinline__ Row make_row(const DiffArgs& a, int b, int kvh, int r, int len) {
+    Row w;
+    w.valid = r < a.R;
+    w.r = w.valid ? r : a.R - 1;
+    const int g = a.G == 1 ? 0 : w.r / a.Nq;
+    w.i = w.r - g * a.Nq;
+    w.h = kvh * a.G + g;
+    w.lim = w.valid ? row_lim(a, len, w.i) : 0;
+    w.at = (size_t)b * a.Nq + w.i;
+    w.st = ((size_t)b * a.H + w.h) * a.Nq + w.i;
+    return w;
+}
+
+// staging of a [32 rows][128 + 128 columns] pair of operands into four [32][64] LDS tiles, registers in between; rows at and behind
+// `rows` are zero
+template <int NT>
+struct Stage {
+    static constexpr int PER = 1024 / NT;
+    u32x4 reg[PER];
+    __device__ __forceinline__ void load(const bf16_t* p0, size_t ld0, const bf16_t* p1, size_t ld1, int row0, int rows, int tid) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int idx = tid + NT * j, row = row0 + (idx >> 5), cc = idx & 31;
+            const bf16_t* src = cc < 16 ? p0 + (size_t)row * ld0 + cc * 8 : p1 + (size_t)row * ld1 + (cc - 16) * 8;
+            reg[j] = row < rows ? *(const u32x4*)src : u32x4{0, 0, 0, 0};
+        }
+    }
+    __device__ __forceinline__ void write(unsigned char* buf, int tid) const {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int idx = tid + NT * j, rl = idx >> 5, cc = idx & 31;
+            *(u32x4*)(buf + (cc >> 3) * TILE + rl * RS + (((cc & 7) ^ swz(rl)) << 4)) = reg[j];
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ forward
+struct FwdOut {
+    bf16_t *out, *o, *o2;     // out [B * Nq, ldo]; o, o2 [B * Nq, H * 128] or NULL
+    size_t ldo;
+    float* lse2;              // [2][B][H][Nq] or NULL
+};
+
+template <int NW>
+__global__ __launch_bounds__(NW * 64, 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * 4 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+    int xb, b, kvh;
+    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+    const int len = clip_len(a, b);
+    const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
+    const Row w = make_row(a, b, kvh, r0 + (lane & 31), len);
+    int wlo = 0, whi = 0, blo, bhi;
+    span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
+    if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
+
+    bf16x8 qf[2][4];
+    const bf16_t* qp = a.q + w.at * a.ldq + (size_t)w.h * HV;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) qf[m][ks] = *(const bf16x8*)(qp + 64 * m + 16 * ks + 8 * hh);
+
+    f32x16 o[2][4];
+    float mx[2], l[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        mx[m] = -__builtin_inff();
+        l[m] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) o[m][dt] = zero16();
+    }
+    const float big = fast_exp2(BIG_LOG2);
+    const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
+    const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
+    const int nkt = (bhi + 31) >> 5;
+    Stage<NW * 64> st;
+    if (nkt > 0) {
+        st.load(kp, a.ldk, vp, a.ldv, 0, len, tid);
+        st.write(smem, tid);
+        __syncthreads();
+    }
+    for (int kt = 0; kt < nkt; ++kt) {
+        const unsigned char* T = smem + (kt & 1) * 4 * TILE;
+        if (kt + 1 < nkt) st.load(kp, a.ldk, vp, a.ldv, (kt + 1) * 32, len, tid);
+        if (kt * 32 < whi) {
+            bf16x8 pf[2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                f32x16 s = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
+                if (kt * 32 + 32 > wlo) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (kt * 32 + acc_row(r, hh) >= w.lim) s[r] = -__builtin_inff();
+                }
+                // the tile is exponentiated against the row's present reference maximum; only a partial sum past 2^20 (the first tile,
+                // with its reference of -inf, always) sends the wave through the exact update
+                float p[16], ls = 0.f, nmc = -mx[m] * a.c;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = fast_exp2(fmaf(s[r], a.c, nmc));
+                    ls += p[r];
+                }
+                const int own = !(ls <= big);
+                if (__any(own)) {
+                    const int trip = own | __shfl_xor(own, 32, 64);
+                    float tm = -__builtin_inff();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[r]);
+                    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+                    const float mn = trip ? fmaxf(mx[m], tm) : mx[m];
+                    const float alpha = trip ? fast_exp2((mx[m] - mn) * a.c) : 1.f;
+                    l[m] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
+                    nmc = -mn * a.c;
+                    ls = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        p[r] = fast_exp2(fmaf(s[r], a.c, nmc));
+                        ls += p[r];
+                    }
+                    mx[m] = mn;
+                }
+                l[m] += ls;
+                pf[m][0] = pack_frag(p, 0);
+                pf[m][1] = pack_frag(p, 1);
+            }
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const bf16x8 vf = tr_frag(T + (2 + (dt >> 1)) * TILE, s2, dt & 1, lane);
+                    o[0][dt] = mfma(vf, pf[0][s2], o[0][dt]);
+                    o[1][dt] = mfma(vf, pf[1][s2], o[1][dt]);
+                }
+        }
+        if (kt + 1 < nkt) st.write(smem + ((kt + 1) & 1) * 4 * TILE, tid);
+        __syncthreads();
+    }
+
+    // epilogue: the two maps' outputs, their difference, its norm
+    float e1, e2, lam = 0.f;
+    const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
+    for (int h = h0; h <= h1; ++h) {
+        const float t = head_lambda(a, h, lane, e1, e2);
+        if (w.h == h) lam = t;
+    }
+    const bool some = w.lim > 0;
+    float inv[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const float lt = l[m] + __shfl_xor(l[m], 32, 64);
+        inv[m] = some ? 1.0f / lt : 0.f;
+        if (f.lse2 && w.valid && hh == 0) f.lse2[(size_t)m * a.B * a.H * a.Nq + w.st] = some ? mx[m] * a.c + fast_log2(lt) : EMPTY_LSE;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[1][dt][r] = some ? o[1][dt][r] * inv[1] : 0.f;
+            const float d = some ? o[0][dt][r] * inv[0] - lam * o[1][dt][r] : 0.f;
+            o[0][dt][r] = d;
+            ss += d * d;
+        }
+    ss += __shfl_xor(ss, 32, 64);
+    if (!w.valid) return;
+    const size_t col = (size_t)w.h * HV;
+    if (f.o) {
+        bf16_t* p = f.o + w.at * a.H * HV + col;
+        bf16_t* p2 = f.o2 + w.at * a.H * HV + col;
+        store_T(p, o[0][0], o[0][1], 1.f, hh);
+        store_T(p + 64, o[0][2], o[0][3], 1.f, hh);
+        store_T(p2, o[1][0], o[1][1], 1.f, hh);
+        store_T(p2 + 64, o[1][2], o[1][3], 1.f, hh);
+    }
+    if (a.gamma) {
+        const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[0][dt][r] *= rn * param(a.gamma, a.param_bf16, 32 * dt + acc_row(r, hh));
+    }
+    bf16_t* y = f.out + w.at * f.ldo + col;
+    store_T(y, o[0][0], o[0][1], 1.f, hh);
+    store_T(y + 64, o[0][2], o[0][3], 1.f, hh);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// Row pass: dO from dY through the norm, the four numbers per row that the two big passes need, and the parameters' gradients.
+//   g = out_scale * gamma * dY, xhat = O / rms, dO = (g - xhat * mean(g xhat)) / rms;  dgamma += out_scale * dY * xhat
+//   d1 = dO . O1, d2 = dO . O2 (O1 = O + lam O2);  dlam -= d2
+// stats[b, h, i] = (lse_1, lse_2 - log2|lam|, d1, sign(lam) d2): the second map's probability comes out of exp2 already times |lam|.
+// 16 lanes a row, a block's rows all of one head; block partials of dgamma / dlam, summed in order by diff_param_kernel.
+__global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t* __restrict__ o, const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dout,
+                                                        size_t lddo, const float* __restrict__ lse2, bf16_t* __restrict__ d_o, f32x4* __restrict__ stats,
+                                                        float* __restrict__ part) {
+    __shared__ float red[16][HV + 1];
+    const int tid = threadIdx.x, lane = tid & 63, sub = tid & 15, slot = tid >> 4, h = blockIdx.y, nb = gridDim.x;
+    float e1, e2;
+    const float lam = head_lambda(a, h, lane, e1, e2);
+    const float loglam = fast_log2(fabsf(lam)), sgn = lam < 0.f ? -1.f : 1.f;
+    float gam[8], dg[8], dl = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        gam[e] = a.gamma ? a.out_scale * param(a.gamma, a.param_bf16, 8 * sub + e) : 1.f;
+        dg[e] = 0.f;
+    }
+    const size_t total = (size_t)a.B * a.Nq, HW = (size_t)a.H * HV, plane = (size_t)a.B * a.H * a.Nq;
+    for (size_t base = (size_t)blockIdx.x * 16; base < total; base += (size_t)nb * 16) {
+        const size_t row = base + slot;
+        if (row >= total) continue;         // whole groups of 16 lanes: the shuffles below stay inside a group
+        const int b = (int)(row / a.Nq), i = (int)(row - (size_t)b * a.Nq);
+        const size_t st = ((size_t)b * a.H + h) * a.Nq + i;
+        const bool some = row_lim(a, clip_len(a, b), i) > 0;
+        const size_t off = row * HW + (size_t)h * HV + 8 * sub;
+        const u32x4 wo = *(const u32x4*)(o + off), w2 = *(const u32x4*)(o2 + off), wd = *(const u32x4*)(dout + row * lddo + (size_t)h * HV + 8 * sub);
+        float vo[8], v2[8], vd[8], gg[8];
+        float ss = 0.f, gx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            vo[e] = (e & 1) ? bf16hi_to_f32(wo[e >> 1]) : bf16lo_to_f32(wo[e >> 1]);
+            v2[e] = (e & 1) ? bf16hi_to_f32(w2[e >> 1]) : bf16lo_to_f32(w2[e >> 1]);
+            vd[e] = (e & 1) ? bf16hi_to_f32(wd[e >> 1]) : bf16lo_to_f32(wd[e >> 1]);
+            gg[e] = gam[e] * vd[e];
+            ss += vo[e] * vo[e];
+            gx += gg[e] * vo[e];
+        }
+        u32x4 rd = wd;
+        if (a.gamma) {
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) {
+                ss += __shfl_xor(ss, x, 64);
+                gx += __shfl_xor(gx, x, 64);
+            }
+            const float rn = 1.0f / sqrtf(ss * (1.f / HV) + a.eps);
+            const float k = gx * rn * rn * (1.f / HV);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                dg[e] += a.out_scale * vd[e] * vo[e] * rn;
+                gg[e] = some ? rn * (gg[e] - vo[e] * k) : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rd[e] = pack_bf16x2(gg[2 * e], gg[2 * e + 1]);
+            *(u32x4*)(d_o + off) = rd;
+        }
+        // d1, d2 from the rounded dO that the products read (their rows then sum to zero as the formula's do); dlam from the unrounded
+        float d1 = 0.f, d2 = 0.f, dx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float q = (e & 1) ? bf16hi_to_f32(rd[e >> 1]) : bf16lo_to_f32(rd[e >> 1]);
+            d1 += q * (vo[e] + lam * v2[e]);
+            d2 += q * v2[e];
+            dx += gg[e] * v2[e];
+        }
+        if (some) dl -= dx;
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) {
+            d1 += __shfl_xor(d1, x, 64);
+            d2 += __shfl_xor(d2, x, 64);
+        }
+        if (sub == 0) stats[st] = some ? f32x4{lse2[st], lse2[plane + st] - loglam, d1, sgn * d2} : f32x4{EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[slot][8 * sub + e] = dg[e];
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) dl += __shfl_xor(dl, x, 64);
+    if (sub == 0) red[slot][HV] = dl;
+    __syncthreads();
+    if (tid <= HV) {
+        float t = 0.f;
+        for (int k = 0; k < 16; ++k) t += red[k][tid];
+        part[((size_t)h * nb + blockIdx.x) * (HV + 1) + tid] = t;
+    }
+}
+
+// block 0 .. lam_heads - 1: the four vectors' gradients of a head (or of all heads); the last block: dgamma
+__global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float* __restrict__ part, int nb, void* dlam, void* dgamma, int grad_bf16) {
+    __shared__ double red[256];
+    const int tid = threadIdx.x;
+    auto put = [&](void* p, size_t i, float v) {
+        if (grad_bf16) ((bf16_t*)p)[i] = f32_to_bf16(v);
+        else ((float*)p)[i] = v;
+    };
+    if ((int)blockIdx.x < a.lam_heads) {
+        const int h0 = a.lam_heads == 1 ? 0 : blockIdx.x, n = (a.lam_heads == 1 ? a.H : 1) * nb;
+        double s = 0.0;
+        for (int k = tid; k < n; k += 256) s += (double)part[((size_t)h0 * nb + k) * (HV + 1) + HV];
+        red[tid] = s;
+        __syncthreads();
+        for (int o = 128; o > 0; o >>= 1) {
+            if (tid < o) red[tid] += red[tid + o];
+            __syncthreads();
+        }
+        const float dl = (float)red[0];
+        float e1, e2;
+        head_lambda(a, blockIdx.x, tid & 63, e1, e2);
+        const int v = tid >> 6;                                    // wave v: vector v; its partner is v ^ 1
+        const size_t st = (size_t)a.lam_heads * 64, at = (size_t)blockIdx.x * 64 + (tid & 63);
+        put(dlam, v * st + at, dl * (v < 2 ? e1 : -e2) * param(a.lam, a.param_bf16, (v ^ 1) * st + at));
+    } else if (dgamma) {
+        const int d = tid & 127, half = tid >> 7, n = a.H * nb;
+        double s = 0.0;
+        for (int k = half; k < n; k += 2) s += (double)part[(size_t)k * (HV + 1) + d];
+        red[tid] = s;
+        __syncthreads();
+        if (half == 0) put(dgamma, d, (float)(red[d] + red[d + 128]));
+    }
+}
+
+// dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability, the sign in d_2)
+template <int NW>
+__global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                             bf16_t* __restrict__ dq, size_t lddq, int nx) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * 4 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+    int xb, b, kvh;
+    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+    const int len = clip_len(a, b);
+    const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
+    const Row w = make_row(a, b, kvh, r0 + (lane & 31), len);
+    int wlo = 0, whi = 0, blo, bhi;
+    span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
+    if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
+    float e1, e2, lam = 0.f;
+    const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
+    for (int h = h0; h <= h1; ++h) {
+        const float t = head_lambda(a, h, lane, e1, e2);
+        if (w.h == h) lam = t;
+    }
+    const float sgn = lam < 0.f ? -1.f : 1.f;
+
+    bf16x8 qf[2][4], of[8];
+    const bf16_t* qp = a.q + w.at * a.ldq + (size_t)w.h * HV;
+    const bf16_t* op = d_o + w.at * lddo + (size_t)w.h * HV;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) qf[m][ks] = *(const bf16x8*)(qp + 64 * m + 16 * ks + 8 * hh);
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) of[ks] = *(const bf16x8*)(op + 16 * ks + 8 * hh);
+    const f32x4 rs = stats[w.st];
+    f32x16 dqa[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
+    const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
+    const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
+    const int nkt = (bhi + 31) >> 5;
+    Stage<NW * 64> st;
+    if (nkt > 0) {
+        st.load(kp, a.ldk, vp, a.ldv, 0, len, tid);
+        st.write(smem, tid);
+        __syncthreads();
+    }
+    for (int kt = 0; kt < nkt; ++kt) {
+        const unsigned char* T = smem + (kt & 1) * 4 * TILE;
+        if (kt + 1 < nkt) st.load(kp, a.ldk, vp, a.ldv, (kt + 1) * 32, len, tid);
+        if (kt * 32 < whi) {
+            f32x16 g = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) g = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), of[ks], g);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                f32x16 s = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
+                float p[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float pr = fast_exp2(fmaf(s[r], a.c, -rs[m]));
+                    p[r] = pr * (m == 0 ? g[r] - rs[2] : fmaf(sgn, g[r], -rs[3]));
+                }
+                if (kt * 32 + 32 > wlo) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (kt * 32 + acc_row(r, hh) >= w.lim) p[r] = 0.f;
+                }
+                const bf16x8 f0 = pack_frag(p, 0), f1 = pack_frag(p, 1);
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) {
+                    dqa[m][dt] = mfma(tr_frag(T + m * TILE, 0, dt, lane), f0, dqa[m][dt]);
+                    dqa[m][dt] = mfma(tr_frag(T + m * TILE, 1, dt, lane), f1, dqa[m][dt]);
+                }
+            }
+        }
+        if (kt + 1 < nkt) st.write(smem + ((kt + 1) & 1) * 4 * TILE, tid);
+        __syncthreads();
+    }
+    if (!w.valid) return;
+    const bool some = w.lim > 0;
+    if (!some) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
+    }
+    bf16_t* y = dq + w.at * lddq + (size_t)w.h * HV;
+    store_T(y, dqa[0][0], dqa[0][1], a.scale, hh);
+    store_T(y + 64, dqa[1][0], dqa[1][1], -a.scale, hh);
+}
+
+// dK, dV: a wave owns 32 keys and walks the query rows of its key head's G heads.  dV = A^T dO with A = P1 - lam P2,
+// dK_1 = scale dS_1^T Q_1, dK_2 = -lam scale dS_2^T Q_2.  Rows that see nothing are staged as zeros, with a log-sum of 1e30.
+template <int NW>
+__global__ __launch_bounds__(NW * 64, 1) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                              bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
+    constexpr int BUF = 4 * TILE + 512;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+    int xb, b, kvh;
+    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+    const int len = clip_len(a, b);
+    const int kb0 = xb * NW * 32, k0 = kb0 + wave * 32, key = k0 + (lane & 31);
+    bf16x8 kf[2][4], vf[8];
+    const size_t krow = (size_t)b * a.Nk + (key < a.Nk ? key : a.Nk - 1);
+    const bf16_t* kp = a.k + krow * a.ldk + (size_t)kvh * HV;
+    const bf16_t* vp = a.v + krow * a.ldv + (size_t)kvh * HV;
+    const u32x4 none = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+        const u32x4 x = key < len ? *(const u32x4*)(kp + 16 * ks + 8 * hh) : none, y = key < len ? *(const u32x4*)(vp + 16 * ks + 8 * hh) : none;
+        kf[ks >> 2][ks & 3] = __builtin_bit_cast(bf16x8, x);
+        vf[ks] = __builtin_bit_cast(bf16x8, y);
+    }
+    f32x16 dva[4], dka[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        dva[i] = zero16();
+        dka[i >> 1][i & 1] = zero16();
+    }
+    const int nqt = (a.Nq + 31) >> 5;
+    // query tiles in which some row sees the block's first key: the limits grow with i
+    int q_first = 0;
+    if (kb0 >= len) q_first = nqt;
+    else if (a.causal) {
+        const int need = (a.causal == 1 ? kb0 : kb0 - (len - a.Nq));      // smallest i with lim(i) > kb0
+        q_first = need > 0 ? need >> 5 : 0;
+        if (q_first > nqt) q_first = nqt;
+    }
+    const int per = nqt - q_first, steps = per * a.G;
+    Stage<NW * 64> st;
+    f32x4 sreg = {0, 0, 0, 0};
+    auto load = [&](int t) {
+        const int g = t / per, qt = q_first + (t - g * per), h = kvh * a.G + g;
+        // first row of the clip that sees anything: earlier ones are staged as zeros through `skip`
+        const bf16_t* qp = a.q + (size_t)b * a.Nq * a.ldq + (size_t)h * HV;
+        const bf16_t* op = d_o + (size_t)b * a.Nq * lddo + (size_t)h * HV;
+        st.load(qp, a.ldq, op, lddo, qt * 32, a.Nq, tid);
+        if (a.causal == 2 && len < a.Nq) {
+#pragma unroll
+            for (int j = 0; j < Stage<NW * 64>::PER; ++j)
+                if (row_lim(a, len, qt * 32 + ((tid + NW * 64 * j) >> 5)) <= 0) st.reg[j] = none;
+        }
+        if (tid < 32) {
+            const int i = qt * 32 + tid;
+            sreg = i < a.Nq ? stats[((size_t)b * a.H + h) * a.Nq + i] : f32x4{EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+        }
+    };
+    auto write = [&](int t) {
+        unsigned char* buf = smem + (t & 1) * BUF;
+        st.write(buf, tid);
+        if (tid < 32) *(f32x4*)(buf + 4 * TILE + tid * 16) = sreg;
+    };
+    if (steps > 0) {
+        load(0);
+        write(0);
+        __syncthreads();
+    }
+    int cur_g = -1;
+    float sgn = 1.f;
+    for (int t = 0; t < steps; ++t) {
+        const int g = t / per, qt = q_first + (t - g * per);
+        if (t + 1 < steps) load(t + 1);
+        if (g != cur_g) {
+            float e1, e2;
+            sgn = head_lambda(a, kvh * a.G + g, lane, e1, e2) < 0.f ? -1.f : 1.f;
+            cur_g = g;
+        }
+        const unsigned char* T = smem + (t & 1) * BUF;
+        const f32x4* S = (const f32x4*)(T + 4 * TILE);
+        const int ilast = min(qt * 32 + 31, a.Nq - 1);
+        if (row_lim(a, len, ilast) > k0) {
+            const bool masked = row_lim(a, len, qt * 32) < k0 + 32;
+            f32x16 gr = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) gr = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), vf[ks], gr);
+            f32x16 s1 = zero16(), s2 = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) s1 = mfma(row_frag(T, ks, lane), kf[0][ks], s1);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) s2 = mfma(row_frag(T + TILE, ks, lane), kf[1][ks], s2);
+            float p1[16], p2[16], A[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const f32x4 rs = S[acc_row(r, hh)];
+                float x1 = fast_exp2(fmaf(s1[r], a.c, -rs[0])), x2 = fast_exp2(fmaf(s2[r], a.c, -rs[1]));
+                if (masked && key >= row_lim(a, len, qt * 32 + acc_row(r, hh))) x1 = x2 = 0.f;
+                A[r] = fmaf(-sgn, x2, x1);
+                p1[r] = x1 * (gr[r] - rs[2]);
+                p2[r] = x2 * fmaf(sgn, gr[r], -rs[3]);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bf16x8 fa = pack_frag(A, s), f1 = pack_frag(p1, s), f2 = pack_frag(p2, s);
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) dva[dt] = mfma(tr_frag(T + (2 + (dt >> 1)) * TILE, s, dt & 1, lane), fa, dva[dt]);
+#pragma unroll
+                for (int dt = 0; dt < 2; ++dt) {
+                    dka[0][dt] = mfma(tr_frag(T, s, dt, lane), f1, dka[0][dt]);
+                    dka[1][dt] = mfma(tr_frag(T + TILE, s, dt, lane), f2, dka[1][dt]);
+                }
+            }
+        }
+        if (t + 1 < steps) write(t + 1);
+        __syncthreads();
+    }
+    if (key >= a.Nk) return;
+    const size_t at = (size_t)b * a.Nk + key;
+    bf16_t* pk = dk + at * lddk + (size_t)kvh * HV;
+    bf16_t* pv = dv + at * lddv + (size_t)kvh * HV;
+    store_T(pk, dka[0][0], dka[0][1], a.scale, hh);
+    store_T(pk + 64, dka[1][0], dka[1][1], -a.scale, hh);
+    store_T(pv, dva[0], dva[1], 1.f, hh);
+    store_T(pv + 64, dva[2], dva[3], 1.f, hh);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int check(const char* who, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
+          const void* lam, int lam_heads, int causal) {
+    if (!q || !k || !v || !lam) MOFO_FAIL(MOFO_EINVAL, "%s: null pointer", who);
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv)
+        MOFO_FAIL(MOFO_EINVAL, "%s: bad dims B=%d Nq=%d Nk=%d H=%d Hkv=%d (H a multiple of Hkv)", who, B, Nq, Nk, H, Hkv);
+    if (H > 4096) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: H=%d (at most 4096)", who, H);
+    if (!(scale > 0.f) || !(scale < 3.0e38f)) MOFO_FAIL(MOFO_EINVAL, "%s: scale must be positive and finite", who);
+    if (lam_heads != 1 && lam_heads != H) MOFO_FAIL(MOFO_EINVAL, "%s: lam of %d heads, must be 1 or H=%d", who, lam_heads, H);
+    if (causal < 0 || causal > 2) MOFO_FAIL(MOFO_EINVAL, "%s: causal=%d must be 0, 1 or 2", who, causal);
+    if (ldq < H * HV || ldk < Hkv * HV || ldv < Hkv * HV || (ldq | ldk | ldv) % 8)
+        MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: bad leading dims ldq=%d ldk=%d ldv=%d (multiples of 8, a row of 128 columns a head)", who, ldq, ldk, ldv);
+    if (ldk > (1 << 24) || ldv > (1 << 24) || ldq > (1 << 24)) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: row pitch above 2^24", who);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: q, k, v must be 16-byte aligned", who);
+    if ((long long)(H / Hkv) * Nq > (1LL << 30) || Nk > (1 << 30)) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: too many rows", who);
+    if ((long long)B * Hkv * (((long long)(H / Hkv) * Nq + Nk) / 32 + 2) > (1LL << 28)) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: grid too large", who);
+    return MOFO_OK;
+}
+
+DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
+                   const void* lam, int lam_heads, float lam_init, const void* gamma, int param_bf16, float eps, float out_scale, const int* kv_len, int causal) {
+    DiffArgs a;
+    a.q = (const bf16_t*)q;
+    a.k = (const bf16_t*)k;
+    a.v = (const bf16_t*)v;
+    a.ldq = (size_t)ldq;
+    a.ldk = (size_t)ldk;
+    a.ldv = (size_t)ldv;
+    a.B = B;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.G = H / Hkv;
+    a.Nq = Nq;
+    a.Nk = Nk;
+    a.R = a.G * Nq;
+    a.causal = causal;
+    a.kv_len = kv_len;
+    a.lam = lam;
+    a.gamma = gamma;
+    a.param_bf16 = param_bf16;
+    a.lam_heads = lam_heads;
+    a.lam_init = lam_init;
+    a.scale = scale;
+    a.c = scale * 1.4426950408889634f;
+    a.eps = eps;
+    a.out_scale = out_scale;
+    return a;
+}
+
+constexpr int FWD_NW = 4;
+unsigned blocks_of(int groups, int nx) { return (unsigned)(8 * ceil_div(groups, 8) * nx); }
+// blocks of one head's rows in the row pass: about 1024 in all, 64 rows each at least
+int row_blocks(int B, int Nq, int H) {
+    const long long rows = (long long)B * Nq;
+    long long nb = (rows + 63) / 64, most = 1024 / H;
+    if (most < 1) most = 1;
+    return (int)(nb < most ? nb : most);
+}
+
+}  // namespace
+
+extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv,
+                                       float scale, const void* lam, int lam_heads, float lam_init, const void* gamma, int param_is_bf16, float eps,
+                                       float out_scale, const int* kv_len, int causal, void* out, int ldo, void* o, void* o2, float* lse2,
+                                       float* ws, long long ws_elems, void* stream) {
+    int rc = check("mofo_diff_attention_fwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal);
+    if (rc) return rc;
+    if (!out) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: null output");
+    if (!o != !o2 || !o != !lse2) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: o, o2 and lse2 go together");
+    if (ldo < H * HV || ldo % 8 || (((uintptr_t)out | (uintptr_t)o | (uintptr_t)o2) & 15))
+        MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_fwd: bad ldo=%d (a multiple of 8), or an output that is not 16-byte aligned", ldo);
+    (void)ws;
+    (void)ws_elems;
+    const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
+    const FwdOut f = {(bf16_t*)out, (bf16_t*)o, (bf16_t*)o2, (size_t)ldo, lse2};
+    const int nx = ceil_div(a.R, 32 * FWD_NW);
+    hipLaunchKernelGGL((diff_fwd_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nx)), dim3(FWD_NW * 64), 0, (hipStream_t)stream, a, f, nx);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd");
+    return MOFO_OK;
+}
+
+extern "C" long long mofo_diff_attention_fwd_ws(int B, int Nq, int Nk, int H, int Hkv) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd_ws: bad dims");
+    return 0;
+}
+
+extern "C" long long mofo_diff_attention_bwd_ws(int B, int Nq, int Nk, int H, int Hkv, int norm) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd_ws: bad dims");
+    const long long rows = (long long)B * Nq * H;
+    return rows * 4 + (norm ? rows * (HV / 2) : 0) + (long long)H * row_blocks(B, Nq, H) * (HV + 1);
+}
+
+extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv,
+                                       float scale, const void* lam, int lam_heads, float lam_init, const void* gamma, int param_is_bf16, float eps,
+                                       float out_scale, const int* kv_len, int causal, const void* o, const void* o2, const float* lse2, const void* dout,
+                                       int lddo, void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, void* dlam, void* dgamma, int grad_is_bf16,
+                                       float* ws, long long ws_elems, void* stream) {
+    int rc = check("mofo_diff_attention_bwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal);
+    if (rc) return rc;
+    if (!o || !o2 || !lse2 || !dout || !dq || !dk || !dv || !dlam || !ws) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: null pointer");
+    if (!gamma != !dgamma) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: gamma and dgamma go together");
+    if (lddo < H * HV || lddq < H * HV || lddk < Hkv * HV || lddv < Hkv * HV || (lddo | lddq | lddk | lddv) % 8)
+        MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: bad leading dims of the gradients");
+    if (((uintptr_t)o | (uintptr_t)o2 | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)
+        MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: tensors must be 16-byte aligned");
+    if (ws_elems < mofo_diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, gamma != nullptr))
+        MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: ws of %lld floats is too small", ws_elems);
+    hipStream_t s = (hipStream_t)stream;
+    const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
+    const size_t rows = (size_t)B * Nq * H;
+    f32x4* stats = (f32x4*)ws;
+    bf16_t* d_o = (bf16_t*)(ws + rows * 4);
+    float* part = ws + rows * 4 + (gamma ? rows * (HV / 2) : 0);
+    const int nb = row_blocks(B, Nq, H);
+    hipLaunchKernelGGL(diff_rows_kernel, dim3(nb, H), dim3(256), 0, s, a, (const bf16_t*)o, (const bf16_t*)o2, (const bf16_t*)dout, (size_t)lddo, lse2, d_o, stats, part);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
+    const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
+    const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
+    const int nx = ceil_div(a.R, 32 * FWD_NW), nk = ceil_div(Nk, 32 * FWD_NW);
+    hipLaunchKernelGGL((diff_dq_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nx)), dim3(FWD_NW * 64), 0, s, a, dy, lddy, stats, (bf16_t*)dq, (size_t)lddq, nx);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dq)");
+    hipLaunchKernelGGL((diff_dkv_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nk)), dim3(FWD_NW * 64), 0, s, a, dy, lddy, stats, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
+                       (size_t)lddv, nk);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dkv)");
+    hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + 1), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(params)");
+    return MOFO_OK;
+}
