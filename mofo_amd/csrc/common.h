@@ -35,6 +35,42 @@ void mofo_set_error(const char* fmt, ...);
         if (e__ != hipSuccess) MOFO_FAIL(MOFO_ELAUNCH, "%s: %s", name, hipGetErrorString(e__)); \
     } while (0)
 
+// A tensor as an entry sees it: `rows` rows of `cols` bytes, `ld` bytes apart.  Column ranges of one packed buffer interleave in memory
+// without sharing an element: with the same pitch, ranges that stay apart within a row do not overlap.
+struct MofoSpan {
+    const char* name;
+    const void* p;
+    long long rows, cols, ld;
+};
+static inline bool mofo_overlap(const MofoSpan& a, const MofoSpan& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.cols <= 0 || b.cols <= 0) return false;
+    const long long a0 = (long long)(uintptr_t)a.p, b0 = (long long)(uintptr_t)b.p;
+    if (a0 + (a.rows - 1) * a.ld + a.cols <= b0 || b0 + (b.rows - 1) * b.ld + b.cols <= a0) return false;
+    const long long ld = a.rows > 1 ? a.ld : b.ld;
+    if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || ld <= 0) return true;
+    const long long off = (((b0 - a0) % ld) + ld) % ld;      // b's first column, seen from a's
+    return !(off >= a.cols && off + b.cols <= ld);
+}
+// the first of outs[0 .. no) that shares memory with one of ins[0 .. ni) or with an earlier output, or -1; the other one's name in *with
+static inline int mofo_overlapping(const MofoSpan* outs, int no, const MofoSpan* ins, int ni, const char** with) {
+    for (int i = 0; i < no; ++i) {
+        for (int j = 0; j < ni + i; ++j) {
+            const MofoSpan& o = j < ni ? ins[j] : outs[j - ni];
+            if (mofo_overlap(outs[i], o)) {
+                *with = o.name;
+                return i;
+            }
+        }
+    }
+    return -1;
+}
+#define MOFO_CHECK_APART(who, outs, no, ins, ni)                                                                     \
+    do {                                                                                                             \
+        const char* with__ = "";                                                                                     \
+        const int bad__ = mofo_overlapping(outs, no, ins, ni, &with__);                                              \
+        if (bad__ >= 0) MOFO_FAIL(MOFO_EINVAL, "%s: %s overlaps %s", who, (outs)[bad__].name, with__);               \
+    } while (0)
+
 // device side -----------------------------------------------------------------------------------
 __device__ __forceinline__ float bf16_to_f32(bf16_t v) { return __uint_as_float(((uint32_t)v) << 16); }
 __device__ __forceinline__ float bf16lo_to_f32(uint32_t w) { return __uint_as_float(w << 16); }

@@ -23,7 +23,11 @@ namespace {
 
 constexpr int HV = 128;                 // columns of a head's q, k, v and output rows
 constexpr float EMPTY_LSE = 1.0e30f;    // log-sum of a row that sees nothing: exp2(s - 1e30) = 0
-constexpr float BIG_LOG2 = 20.f;        // forward: a row's reference maximum is kept until a tile's partial sum passes 2^20
+// Forward: a row's reference maximum is kept until a score lies more than this many log2 units above it.  The row's outputs are divided
+// by the sum of the ROUNDED terms, so that the rounding of a term that dominates its row cancels; the reference follows a term that is
+// far above it, which is then 1 and not rounded at all.  (Gradients are formed from differences G - d in which such a term cancels: with
+// the sum of the unrounded terms and a reference kept up to 2^20, dq of 160 and 50 tokens was 6e-3 and 1e-2 off; this way 3e-3.)
+constexpr float KEEP_REF = 5.f;
 
 struct DiffArgs {
     const bf16_t *q, *k, *v;
@@ -57,6 +61,13 @@ __device__ __forceinline__ void span_lim(const DiffArgs& a, int len, int ra, int
     hi = row_lim(a, len, one ? rb % a.Nq : a.Nq - 1);
 }
 __device__ __forceinline__ float param(const void* p, int bf, size_t i) { return bf ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i]; }
+__device__ __forceinline__ f32x4 gamma4(const DiffArgs& a, int d) {
+    if (a.param_bf16) {
+        const u32x2 w = *(const u32x2*)((const bf16_t*)a.gamma + d);
+        return f32x4{bf16lo_to_f32(w[0]), bf16hi_to_f32(w[0]), bf16lo_to_f32(w[1]), bf16hi_to_f32(w[1])};
+    }
+    return *(const f32x4*)((const float*)a.gamma + d);
+}
 // lambda of head h, and its two exponentials (every lane of the wave)
 __device__ __forceinline__ float head_lambda(const DiffArgs& a, int h, int lane, float& e1, float& e2) {
     const int hl = a.lam_heads == 1 ? 0 : h;
@@ -71,20 +82,18 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 acc) { return 
 // one lane's row of a wave tile
 struct Row {
     bool valid;
-    int r, h, i, lim;
-    size_t at;      // row of q / out / dout: b * Nq + i
-    size_t st;      // index into the [B, H, Nq] statistics
+    int h, i, lim;
 };
-__device__ __forceinline__ Row make_row(const DiffArgs& a, int b, int kvh, int r, int len) {
+__device__ __forceinline__ size_t row_at(const DiffArgs& a, int b, const Row& w) { return (size_t)b * a.Nq + w.i; }                       // of q, out, dout
+__device__ __forceinline__ size_t stat_at(const DiffArgs& a, int b, const Row& w) { return ((size_t)b * a.H + w.h) * a.Nq + w.i; }    // of [B, H, Nq]
+__device__ __forceinline__ Row make_row(const DiffArgs& a, int kvh, int r, int len) {
     Row w;
     w.valid = r < a.R;
-    w.r = w.valid ? r : a.R - 1;
-    const int g = a.G == 1 ? 0 : w.r / a.Nq;
-    w.i = w.r - g * a.Nq;
+    if (!w.valid) r = a.R - 1;
+    const int g = a.G == 1 ? 0 : r / a.Nq;
+    w.i = r - g * a.Nq;
     w.h = kvh * a.G + g;
     w.lim = w.valid ? row_lim(a, len, w.i) : 0;
-    w.at = (size_t)b * a.Nq + w.i;
-    w.st = ((size_t)b * a.H + w.h) * a.Nq + w.i;
     return w;
 }
 
@@ -111,161 +120,318 @@ struct Stage {
     }
 };
 
+// LDS-DMA of one operand's [32 rows][64 columns] half tile, as four pieces of 8 rows: rows at and behind `rows` come from a line of zeros
+__device__ const u32x4 g_zero = {0, 0, 0, 0};
+struct HalfTile {
+    const bf16_t* base;     // first row's 64 columns
+    size_t ld;
+    int voff[2];            // byte offset of the lane's 16 bytes inside an even / odd piece (the swizzle sits on the source column)
+};
+__device__ __forceinline__ HalfTile half_tile(const bf16_t* base, size_t ld, int lane) {
+    HalfTile t;
+    t.base = base;
+    t.ld = ld;
+#pragma unroll
+    for (int o = 0; o < 2; ++o) t.voff[o] = (int)(((size_t)(lane >> 3) * ld + (((lane & 7) ^ swz(8 * o + (lane >> 3))) << 3)) * 2);
+    return t;
+}
+__device__ __forceinline__ void dma_piece(const void* sbase, int voff, unsigned lds_dst) {
+    unsigned keep;
+    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(sbase), "s"(lds_dst)
+                 : "memory");
+}
+__device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane) {
+    if (row0 + 32 <= rows) {
+        const char* p = (const char*)(t.base + (size_t)row0 * t.ld);
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) dma_piece(p + (size_t)sub * 16 * t.ld, t.voff[sub & 1], lds_dst + sub * 1024);
+    } else {
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) {
+            const int rl = 8 * sub + (lane >> 3), row = row0 + rl;
+            const void* src = row < rows ? (const void*)(t.base + (size_t)row * t.ld + (((lane & 7) ^ swz(rl)) << 3)) : (const void*)&g_zero;
+            dma_b128(src, lds_dst + sub * 1024);
+        }
+    }
+}
+// own pieces but the N newest have landed, own LDS reads are done; then every wave's
+template <int N>
+__device__ __forceinline__ void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 struct FwdOut {
     bf16_t *out, *o, *o2;     // out [B * Nq, ldo]; o, o2 [B * Nq, H * 128] or NULL
     size_t ldo;
     float* lse2;              // [2][B][H][Nq] or NULL
+    float* part;              // nsplit > 1: [rows][nsplit][2][128] outputs of a range of keys, divided by its own sum, then
+    float* part_lse;          // [rows][nsplit][2] its log2-sum (-inf: nothing seen); rows = B * H * Nq
 };
 
-template <int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * 4 * TILE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
-    int xb, b, kvh;
-    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+// sum of the eight rounded terms of a fragment
+__device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    const u32x4 w = __builtin_bit_cast(u32x4, f);
+    const bf16x2 one = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t pair = w[e];       // (a bit cast of the vector's element itself reads element 0)
+        acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, acc, false);
+    }
+    return acc;
+}
+
+// One block: NW waves of 32 rows that share the key tiles of one (clip, key head), or of a range of them (nsplit > 1, few blocks).  The
+// tiles go through a ring of three LDS stages, filled by LDS-DMA two stages ahead, one barrier a tile.
+template <int NW, bool SAVE, bool SPLIT>
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit) {
+    constexpr int STAGE = 4 * TILE, PIECES = 16 / NW;     // LDS-DMA pieces a wave issues per stage
+    __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int xs, b, kvh;
+    if (!decode_block(nx * nsplit, a.B * a.Hkv, a.Hkv, xs, b, kvh)) return;
+    const int xb = xs / nsplit, sp = xs - xb * nsplit;
     const int len = clip_len(a, b);
     const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
-    const Row w = make_row(a, b, kvh, r0 + (lane & 31), len);
+    const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
     span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
+    // this block's range of key tiles
+    const int tiles = (bhi + 31) >> 5, chunk = (tiles + nsplit - 1) / nsplit;
+    const int t0 = min(sp * chunk, tiles), t1 = min(t0 + chunk, tiles), nkt = t1 - t0;
+
+    HalfTile ht[4 / NW > 0 ? 4 / NW : 1];
+    const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
+    const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
+#pragma unroll
+    for (int j = 0; j < 4 / NW; ++j) {
+        const int ti = wave * (4 / NW) + j;               // K_1, K_2, V columns 0..63, 64..127
+        ht[j] = half_tile((ti < 2 ? kp : vp) + (ti & 1) * 64, ti < 2 ? a.ldk : a.ldv, lane);
+    }
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    auto issue = [&](int t, unsigned buf) {
+#pragma unroll
+        for (int j = 0; j < 4 / NW; ++j) dma_half_tile(ht[j], (t0 + t) * 32, len, lds0 + buf * STAGE + (wave * (4 / NW) + j) * TILE, lane);
+    };
+    if (nkt > 0) issue(0, 0);
+    if (nkt > 1) issue(1, 1);
 
     bf16x8 qf[2][4];
-    const bf16_t* qp = a.q + w.at * a.ldq + (size_t)w.h * HV;
+    const bf16_t* qp = a.q + row_at(a, b, w) * a.ldq + (size_t)w.h * HV;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) qf[m][ks] = *(const bf16x8*)(qp + 64 * m + 16 * ks + 8 * hh);
 
     f32x16 o[2][4];
-    float mx[2], l[2];
+    float mx[2], l[2], le[2];          // reference maximum, sum of the rounded terms, sum of the unrounded terms (SAVE)
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         mx[m] = -__builtin_inff();
-        l[m] = 0.f;
+        l[m] = le[m] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) o[m][dt] = zero16();
     }
-    const float big = fast_exp2(BIG_LOG2);
-    const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
-    const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
-    const int nkt = (bhi + 31) >> 5;
-    Stage<NW * 64> st;
-    if (nkt > 0) {
-        st.load(kp, a.ldk, vp, a.ldv, 0, len, tid);
-        st.write(smem, tid);
-        __syncthreads();
-    }
-    for (int kt = 0; kt < nkt; ++kt) {
-        const unsigned char* T = smem + (kt & 1) * 4 * TILE;
-        if (kt + 1 < nkt) st.load(kp, a.ldk, vp, a.ldv, (kt + 1) * 32, len, tid);
-        if (kt * 32 < whi) {
-            bf16x8 pf[2][2];
+
+    const float keep = KEEP_REF / a.c;                    // in score units
+    int buf = 0;
+    for (int t = 0; t < nkt; ++t) {
+        if (t + 1 < nkt) landed_barrier<PIECES>();
+        else landed_barrier<0>();
+        if (t + 2 < nkt) issue(t + 2, buf == 0 ? 2 : buf - 1);
+        const int k0 = (t0 + t) * 32;
+        const unsigned char* T = smem + buf * STAGE;
+        buf = buf == 2 ? 0 : buf + 1;
+        if (k0 >= whi) continue;                          // no row of this wave sees the tile
+        bf16x8 pf[2][2];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                f32x16 s = zero16();
+        for (int m = 0; m < 2; ++m) {
+            f32x16 s = zero16();
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
-                if (kt * 32 + 32 > wlo) {
+            for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
+            if (k0 + 32 > wlo) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (kt * 32 + acc_row(r, hh) >= w.lim) s[r] = -__builtin_inff();
-                }
-                // the tile is exponentiated against the row's present reference maximum; only a partial sum past 2^20 (the first tile,
-                // with its reference of -inf, always) sends the wave through the exact update
-                float p[16], ls = 0.f, nmc = -mx[m] * a.c;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    p[r] = fast_exp2(fmaf(s[r], a.c, nmc));
-                    ls += p[r];
-                }
-                const int own = !(ls <= big);
-                if (__any(own)) {
-                    const int trip = own | __shfl_xor(own, 32, 64);
-                    float tm = -__builtin_inff();
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[r]);
-                    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-                    const float mn = trip ? fmaxf(mx[m], tm) : mx[m];
-                    const float alpha = trip ? fast_exp2((mx[m] - mn) * a.c) : 1.f;
-                    l[m] *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
-                    nmc = -mn * a.c;
-                    ls = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        p[r] = fast_exp2(fmaf(s[r], a.c, nmc));
-                        ls += p[r];
-                    }
-                    mx[m] = mn;
-                }
-                l[m] += ls;
-                pf[m][0] = pack_frag(p, 0);
-                pf[m][1] = pack_frag(p, 1);
+                for (int r = 0; r < 16; ++r)
+                    if (k0 + acc_row(r, hh) >= w.lim) s[r] = -__builtin_inff();
             }
+            float tm = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) tm = fmaxf(tm, s[r]);
+            if (__any(tm > mx[m] + keep)) {               // the first tile (reference -inf) too
+                tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+                const float mn = tm > mx[m] + keep ? tm : mx[m];
+                const float alpha = tm > mx[m] + keep ? fast_exp2((mx[m] - mn) * a.c) : 1.f;
+                mx[m] = mn;
+                l[m] *= alpha;
+                if constexpr (SAVE) le[m] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
+            }
+            const float nmc = -mx[m] * a.c;
+#pragma unroll
+            for (int h8 = 0; h8 < 2; ++h8) {
+                float p[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    p[r] = fast_exp2(fmaf(s[8 * h8 + r], a.c, nmc));
+                    if constexpr (SAVE) le[m] += p[r];
+                }
+                pf[m][h8] = pack_frag(p, 0);
+                l[m] = frag_sum(pf[m][h8], l[m]);
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const bf16x8 vf = tr_frag(T + (2 + (dt >> 1)) * TILE, s2, dt & 1, lane);
+                o[0][dt] = mfma(vf, pf[0][s2], o[0][dt]);
+                o[1][dt] = mfma(vf, pf[1][s2], o[1][dt]);
+            }
+    }
+
+    const bool some = w.lim > t0 * 32 && nkt > 0;          // the row sees a key of this range
+    float inv[2], lse[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const float lt = l[m] + __shfl_xor(l[m], 32, 64);
+        const float lx = SAVE ? le[m] + __shfl_xor(le[m], 32, 64) : lt;
+        inv[m] = some ? 1.0f / lt : 0.f;
+        lse[m] = mx[m] * a.c + fast_log2(lx);
+    }
+    if constexpr (SPLIT) {
+        if (!w.valid) return;
+        const size_t pi = stat_at(a, b, w) * nsplit + sp;
+        float* pp = f.part + pi * (2 * HV);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    const bf16x8 vf = tr_frag(T + (2 + (dt >> 1)) * TILE, s2, dt & 1, lane);
-                    o[0][dt] = mfma(vf, pf[0][s2], o[0][dt]);
-                    o[1][dt] = mfma(vf, pf[1][s2], o[1][dt]);
+                for (int rg = 0; rg < 4; ++rg) {
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = some ? o[m][dt][4 * rg + e] * inv[m] : 0.f;
+                    *(f32x4*)(pp + m * HV + 32 * dt + 8 * rg + 4 * hh) = x;
                 }
+            if (hh == 0) f.part_lse[pi * 2 + m] = some ? lse[m] : -__builtin_inff();
         }
-        if (kt + 1 < nkt) st.write(smem + ((kt + 1) & 1) * 4 * TILE, tid);
-        __syncthreads();
-    }
-
-    // epilogue: the two maps' outputs, their difference, its norm
+    } else {
     float e1, e2, lam = 0.f;
     const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
     for (int h = h0; h <= h1; ++h) {
         const float t = head_lambda(a, h, lane, e1, e2);
         if (w.h == h) lam = t;
     }
-    const bool some = w.lim > 0;
-    float inv[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        const float lt = l[m] + __shfl_xor(l[m], 32, 64);
-        inv[m] = some ? 1.0f / lt : 0.f;
-        if (f.lse2 && w.valid && hh == 0) f.lse2[(size_t)m * a.B * a.H * a.Nq + w.st] = some ? mx[m] * a.c + fast_log2(lt) : EMPTY_LSE;
-    }
+    const size_t col = (size_t)w.h * HV, own = row_at(a, b, w) * a.H * HV + col + 4 * hh;
     float ss = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 4; ++dt) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            o[1][dt][r] = some ? o[1][dt][r] * inv[1] : 0.f;
-            const float d = some ? o[0][dt][r] * inv[0] - lam * o[1][dt][r] : 0.f;
-            o[0][dt][r] = d;
-            ss += d * d;
+        for (int rg = 0; rg < 4; ++rg) {
+            float x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = some ? o[1][dt][4 * rg + e] * inv[1] : 0.f;
+                x[e] = some ? fmaf(-lam, y[e], o[0][dt][4 * rg + e] * inv[0]) : 0.f;
+                ss = fmaf(x[e], x[e], ss);
+                o[0][dt][4 * rg + e] = x[e];
+            }
+            if constexpr (SAVE) {
+                if (w.valid) {
+                    *(u32x2*)(f.o + own + 32 * dt + 8 * rg) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+                    *(u32x2*)(f.o2 + own + 32 * dt + 8 * rg) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);            // everything at once does not fit beside the accumulators
         }
+    }
     ss += __shfl_xor(ss, 32, 64);
     if (!w.valid) return;
-    const size_t col = (size_t)w.h * HV;
-    if (f.o) {
-        bf16_t* p = f.o + w.at * a.H * HV + col;
-        bf16_t* p2 = f.o2 + w.at * a.H * HV + col;
-        store_T(p, o[0][0], o[0][1], 1.f, hh);
-        store_T(p + 64, o[0][2], o[0][3], 1.f, hh);
-        store_T(p2, o[1][0], o[1][1], 1.f, hh);
-        store_T(p2 + 64, o[1][2], o[1][3], 1.f, hh);
+    if constexpr (SAVE) {
+        if (hh == 0) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) f.lse2[(size_t)m * a.B * a.H * a.Nq + stat_at(a, b, w)] = some ? lse[m] : EMPTY_LSE;
+        }
     }
     if (a.gamma) {
         const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int dt = 0; dt < 4; ++dt) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[0][dt][r] *= rn * param(a.gamma, a.param_bf16, 32 * dt + acc_row(r, hh));
+            for (int rg = 0; rg < 4; ++rg) {
+                const f32x4 g = gamma4(a, 32 * dt + 8 * rg + 4 * hh);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[0][dt][4 * rg + e] *= rn * g[e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    bf16_t* y = f.out + w.at * f.ldo + col;
+    bf16_t* y = f.out + row_at(a, b, w) * f.ldo + col;
     store_T(y, o[0][0], o[0][1], 1.f, hh);
     store_T(y + 64, o[0][2], o[0][3], 1.f, hh);
+    }
+}
+
+// joins the ranges of a row: one wave a row, lanes 0..31 the first map's 128 columns, lanes 32..63 the second's; the ranges' weights are
+// exp2(lse_range - lse), lane s holding range s
+__global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, int nsplit) {
+    const int lane = threadIdx.x & 63, m = lane >> 5, d = (lane & 31) * 4;
+    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (size_t)a.B * a.H * a.Nq;
+    if (row >= rows) return;
+    const size_t bh = row / a.Nq;
+    const int i = (int)(row - bh * a.Nq), b = (int)(bh / a.H), h = (int)(bh - (size_t)b * a.H);
+    float e1, e2;
+    const float lam = head_lambda(a, h, lane, e1, e2);
+    float wgt[2], lse[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const float x = lane < nsplit ? f.part_lse[(row * nsplit + lane) * 2 + n] : -__builtin_inff();
+        const float top = wave_max(x), e = top == -__builtin_inff() ? 0.f : fast_exp2(x - top), sum = wave_sum(e);
+        wgt[n] = sum > 0.f || sum != sum ? e / sum : 0.f;
+        lse[n] = sum > 0.f || sum != sum ? top + fast_log2(sum) : EMPTY_LSE;
+    }
+    const float* pp = f.part + row * nsplit * (2 * HV) + m * HV + d;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int s = 0; s < nsplit; ++s) {
+        const f32x4 x = *(const f32x4*)(pp + (size_t)s * (2 * HV));
+        // lane s holds range s's weight of both maps
+        const float w0 = __shfl(wgt[0], s, 64), w1 = __shfl(wgt[1], s, 64), w = m ? w1 : w0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += w * x[e];
+    }
+    f32x4 o2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o2[e] = __shfl_xor(acc[e], 32, 64);
+    float ss = 0.f;
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o[e] = acc[e] - lam * o2[e];                      // of use in lanes 0..31
+        ss += o[e] * o[e];
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) ss += __shfl_xor(ss, x, 64);
+    const size_t at = ((size_t)b * a.Nq + i), off = at * a.H * HV + (size_t)h * HV + d;
+    if (f.o && m) *(u32x2*)(f.o2 + off) = u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    if (m) return;
+    if (f.o) {
+        *(u32x2*)(f.o + off) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+        if (lane < 2) f.lse2[(size_t)lane * rows + row] = lane ? lse[1] : lse[0];
+    }
+    if (a.gamma) {
+        const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= rn * param(a.gamma, a.param_bf16, d + e);
+    }
+    *(u32x2*)(f.out + at * f.ldo + (size_t)h * HV + d) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -400,7 +566,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
     if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
     const int len = clip_len(a, b);
     const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
-    const Row w = make_row(a, b, kvh, r0 + (lane & 31), len);
+    const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
     span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
@@ -413,15 +579,15 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
     const float sgn = lam < 0.f ? -1.f : 1.f;
 
     bf16x8 qf[2][4], of[8];
-    const bf16_t* qp = a.q + w.at * a.ldq + (size_t)w.h * HV;
-    const bf16_t* op = d_o + w.at * lddo + (size_t)w.h * HV;
+    const bf16_t* qp = a.q + row_at(a, b, w) * a.ldq + (size_t)w.h * HV;
+    const bf16_t* op = d_o + row_at(a, b, w) * lddo + (size_t)w.h * HV;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) qf[m][ks] = *(const bf16x8*)(qp + 64 * m + 16 * ks + 8 * hh);
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) of[ks] = *(const bf16x8*)(op + 16 * ks + 8 * hh);
-    const f32x4 rs = stats[w.st];
+    const f32x4 rs = stats[stat_at(a, b, w)];
     f32x16 dqa[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
@@ -474,7 +640,7 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
 #pragma unroll
         for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
     }
-    bf16_t* y = dq + w.at * lddq + (size_t)w.h * HV;
+    bf16_t* y = dq + row_at(a, b, w) * lddq + (size_t)w.h * HV;
     store_T(y, dqa[0][0], dqa[0][1], a.scale, hh);
     store_T(y + 64, dqa[1][0], dqa[1][1], -a.scale, hh);
 }
@@ -655,6 +821,26 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
 
 constexpr int FWD_NW = 4;
 unsigned blocks_of(int groups, int nx) { return (unsigned)(8 * ceil_div(groups, 8) * nx); }
+// Waves per block and split of the keys.  Few rows: one block a 32- or 64-row list.  Fewer blocks than the card holds (two of 128 rows a
+// compute unit, three of 32): the keys of each are cut into ranges of at least two tiles, as many as fill it; at most 64 ranges, and
+// 65536 partial rows.
+constexpr int PART = 2 * HV + 2;        // floats of workspace per row and range
+struct FwdPlan {
+    int nw, nx, nsplit;
+};
+FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv) {
+    FwdPlan p;
+    const long long R = (long long)(H / Hkv) * Nq, rows = (long long)B * H * Nq;
+    p.nw = R <= 32 ? 1 : R <= 64 ? 2 : 4;
+    p.nx = (int)((R + 32 * p.nw - 1) / (32 * p.nw));
+    const long long blocks = (long long)B * Hkv * p.nx, room = 256 * (p.nw == 4 ? 2 : 3), tiles = (Nk + 31) / 32;
+    long long n = room / blocks;
+    if (n > (tiles + 1) / 2) n = (tiles + 1) / 2;
+    if (n > 64) n = 64;
+    if (n > 65536 / rows) n = 65536 / rows;
+    p.nsplit = n < 2 ? 1 : (int)n;
+    return p;
+}
 // blocks of one head's rows in the row pass: about 1024 in all, 64 rows each at least
 int row_blocks(int B, int Nq, int H) {
     const long long rows = (long long)B * Nq;
@@ -675,19 +861,49 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
     if (!o != !o2 || !o != !lse2) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: o, o2 and lse2 go together");
     if (ldo < H * HV || ldo % 8 || (((uintptr_t)out | (uintptr_t)o | (uintptr_t)o2) & 15))
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_fwd: bad ldo=%d (a multiple of 8), or an output that is not 16-byte aligned", ldo);
-    (void)ws;
-    (void)ws_elems;
+    const FwdPlan pl = fwd_plan(B, Nq, Nk, H, Hkv);
+    const long long rows = (long long)B * H * Nq;
+    if (pl.nsplit > 1 && (!ws || ws_elems < rows * pl.nsplit * PART)) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: ws of %lld floats is too small", ws ? ws_elems : 0);
+    if (pl.nsplit > 1 && ((uintptr_t)ws & 15)) MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_fwd: ws must be 16-byte aligned");
+    {
+        const long long HW = (long long)H * HV * 2, KW = (long long)Hkv * HV * 2, Mq = (long long)B * Nq, Mk = (long long)B * Nk, es = param_is_bf16 ? 2 : 4;
+        const MofoSpan outs[] = {{"out", out, Mq, HW, 2LL * ldo}, {"o", o, 1, Mq * HW, 0}, {"o2", o2, 1, Mq * HW, 0}, {"lse2", lse2, 1, 8 * Mq * H, 0},
+                                 {"ws", pl.nsplit > 1 ? ws : nullptr, 1, rows * pl.nsplit * PART * 4, 0}};
+        const MofoSpan in[] = {{"q", q, Mq, HW, 2LL * ldq}, {"k", k, Mk, KW, 2LL * ldk}, {"v", v, Mk, KW, 2LL * ldv}, {"lam", lam, 1, 256LL * lam_heads * es, 0},
+                               {"gamma", gamma, 1, HV * es, 0}, {"kv_len", kv_len, 1, 4LL * B, 0}};
+        MOFO_CHECK_APART("mofo_diff_attention_fwd", outs, 5, in, 6);
+    }
     const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
-    const FwdOut f = {(bf16_t*)out, (bf16_t*)o, (bf16_t*)o2, (size_t)ldo, lse2};
-    const int nx = ceil_div(a.R, 32 * FWD_NW);
-    hipLaunchKernelGGL((diff_fwd_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nx)), dim3(FWD_NW * 64), 0, (hipStream_t)stream, a, f, nx);
+    FwdOut f = {(bf16_t*)out, (bf16_t*)o, (bf16_t*)o2, (size_t)ldo, lse2, nullptr, nullptr};
+    if (pl.nsplit > 1) {
+        f.part = ws;
+        f.part_lse = ws + rows * pl.nsplit * (2 * HV);
+    }
+    const dim3 grid(blocks_of(B * Hkv, pl.nx * pl.nsplit));
+    hipStream_t s = (hipStream_t)stream;
+#define MOFO_DIFF_FWD(NW)                                                                                                          \
+    do {                                                                                                                           \
+        if (o && pl.nsplit > 1) hipLaunchKernelGGL((diff_fwd_kernel<NW, true, true>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, pl.nsplit);  \
+        else if (o) hipLaunchKernelGGL((diff_fwd_kernel<NW, true, false>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, 1);               \
+        else if (pl.nsplit > 1) hipLaunchKernelGGL((diff_fwd_kernel<NW, false, true>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, pl.nsplit); \
+        else hipLaunchKernelGGL((diff_fwd_kernel<NW, false, false>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, 1);                     \
+    } while (0)
+    if (pl.nw == 1) MOFO_DIFF_FWD(1);
+    else if (pl.nw == 2) MOFO_DIFF_FWD(2);
+    else MOFO_DIFF_FWD(4);
+#undef MOFO_DIFF_FWD
     MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd");
+    if (pl.nsplit > 1) {
+        hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, f, pl.nsplit);
+        MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd(join)");
+    }
     return MOFO_OK;
 }
 
 extern "C" long long mofo_diff_attention_fwd_ws(int B, int Nq, int Nk, int H, int Hkv) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd_ws: bad dims");
-    return 0;
+    const FwdPlan pl = fwd_plan(B, Nq, Nk, H, Hkv);
+    return pl.nsplit > 1 ? (long long)B * H * Nq * pl.nsplit * PART : 0;
 }
 
 extern "C" long long mofo_diff_attention_bwd_ws(int B, int Nq, int Nk, int H, int Hkv, int norm) {
@@ -711,6 +927,16 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: tensors must be 16-byte aligned");
     if (ws_elems < mofo_diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, gamma != nullptr))
         MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: ws of %lld floats is too small", ws_elems);
+    {
+        const long long HW = (long long)H * HV * 2, KW = (long long)Hkv * HV * 2, Mq = (long long)B * Nq, Mk = (long long)B * Nk, es = param_is_bf16 ? 2 : 4,
+                        eg = grad_is_bf16 ? 2 : 4;
+        const MofoSpan outs[] = {{"dq", dq, Mq, HW, 2LL * lddq}, {"dk", dk, Mk, KW, 2LL * lddk}, {"dv", dv, Mk, KW, 2LL * lddv}, {"dlam", dlam, 1, 256LL * lam_heads * eg, 0},
+                                 {"dgamma", dgamma, 1, HV * eg, 0}, {"ws", ws, 1, mofo_diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, gamma != nullptr) * 4, 0}};
+        const MofoSpan in[] = {{"q", q, Mq, HW, 2LL * ldq}, {"k", k, Mk, KW, 2LL * ldk}, {"v", v, Mk, KW, 2LL * ldv}, {"lam", lam, 1, 256LL * lam_heads * es, 0},
+                               {"gamma", gamma, 1, HV * es, 0}, {"kv_len", kv_len, 1, 4LL * B, 0}, {"o", o, 1, Mq * HW, 0}, {"o2", o2, 1, Mq * HW, 0},
+                               {"lse2", lse2, 1, 8 * Mq * H, 0}, {"dout", dout, Mq, HW, 2LL * lddo}};
+        MOFO_CHECK_APART("mofo_diff_attention_bwd", outs, 6, in, 10);
+    }
     hipStream_t s = (hipStream_t)stream;
     const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
     const size_t rows = (size_t)B * Nq * H;

@@ -143,6 +143,13 @@ extern "C" int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, 
     if (ldx < W || ldo < W || ldx % vec || ldo % vec || ((uintptr_t)x & 15) || ((uintptr_t)out & 15))
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_rope_axes: rows of 16-byte aligned pieces (ldx=%d, ldo=%d for %lld columns)", ldx, ldo, W);
     if (x == out && ldx != ldo) MOFO_FAIL(MOFO_EINVAL, "mofo_rope_axes: in place with two row pitches (%d, %d)", ldx, ldo);
+    {
+        const int es = x_is_bf16 ? 2 : 4;
+        const MofoSpan o = {"out", out, M, W * es, (long long)ldo * es};
+        const MofoSpan in[] = {{"x", x == out ? nullptr : x, M, W * es, (long long)ldx * es}, {"freqs", freqs, 1, pairs * 8, 0},
+                               {"pos", pos, 1, (long long)M * naxes * 4, 0}, {"tok_idx", tok_idx, 1, (long long)M * 4, 0}};
+        MOFO_CHECK_APART("mofo_rope_axes", &o, 1, in, 4);
+    }
     RopeArgs a;
     a.x = x;
     a.out = out;

@@ -509,43 +509,20 @@ def attention_bwd_dkv(qkv, dout, lse2, delta, B, N, H, scale, dqkv, q_begin=0):
 
 
 # ------------------------------------------------------------------------------------------------ rotary positions, differential attention
-def _together(*ts):
-    """all tensors (None left out) on ONE device, and that the current one: the launch goes to the current device's stream"""
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.device.index != dev:
-            raise ValueError(f"tensors must be on the current device cuda:{dev}, got one on {t.device}")
+# (the entries refuse overlapping tensors and rows that do not start at multiples of 16 bytes; here types, shapes, contiguity and the device)
+def _dev_chk(dev, dtype, dims, **tensors):
+    """every tensor (None left out) has this type, this many dims, a contiguous last dim, and lies on the current device, to whose stream the
+    launch goes"""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev or t.dim() != dims or t.stride(-1) != 1):
+            _chk(t, dtype, name, dims)
+            if t.get_device() != dev:
+                raise ValueError(f"{name} must be on the current device cuda:{dev}, it is on {t.device}")
 
 
-def _span(t):
-    n = t.numel()
-    return t.data_ptr(), t.data_ptr() + ((sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size() if n else 0)
-
-
-def _overlap(a, b):
-    """do two row-major tensors share an element?  Column ranges of one packed buffer (the same row pitch) do not."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    if a.dim() == 2 and b.dim() == 2 and a.stride(0) == b.stride(0) and a.element_size() == b.element_size() and a.shape[0] > 1:
-        ld, e = a.stride(0), a.element_size()
-        off = ((b0 - a0) // e) % ld
-        return (b0 - a0) % e != 0 or not (off >= a.shape[1] and off + b.shape[1] <= ld)
-    return True
-
-
-def _apart(outs, ins, who):
-    for i, (n, o) in enumerate(outs):
-        if o is None:
-            continue
-        for m, t in ins + outs[:i]:
-            if t is not None and _overlap(o, t):
-                raise ValueError(f"{who}: {n} overlaps {m}")
-
-
-def _rows16(t, name):
-    if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) * t.element_size() % 16):
-        raise ValueError(f"{name}: rows must start at multiples of 16 bytes")
+def _ld16(t):
+    """row pitch of a 2-D tensor; a single row's own stride says nothing"""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def rope_freqs(sections, base=10000.0, device="cuda"):
@@ -554,48 +531,40 @@ def rope_freqs(sections, base=10000.0, device="cuda"):
     return torch.tensor([base ** (-i / n) / (2 * math.pi) for n in sections for i in range(n)], dtype=torch.float64, device=device)
 
 
-def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, interleaved, inverse, names):
+def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, interleaved, inverse, nx, nout):
     if x is None or x.dtype not in (F32, BF16):
-        raise TypeError(f"{names[0]} must be f32 or bf16")
-    _chk(x, x.dtype, names[0], 2), _chk(out, x.dtype, names[1], 2), _chk(freqs, torch.float64, "freqs", 1)
-    M = x.shape[0]
-    sections = [int(n) for n in sections]
-    if not 1 <= len(sections) <= 4 or min(sections) < 0:
+        raise TypeError(f"{nx} must be f32 or bf16")
+    dt, dev = x.dtype, torch.cuda.current_device() if x.is_cuda else -1
+    _dev_chk(dev, dt, 2, **{nx: x, nout: out})
+    _dev_chk(dev, torch.float64, 1, freqs=freqs)
+    if not x.is_cuda or out is None or freqs is None:
+        _chk(x, dt, nx), _chk(out, dt, nout), _chk(freqs, torch.float64, "freqs")
+    M, axes = x.shape[0], len(sections)
+    if not 1 <= axes <= 4 or min(sections) < 0:
         raise ValueError("rope_axes: one to four sections, none negative")
     pairs = sum(sections)
     if x.shape[1] != heads * head_dim or out.shape != x.shape:
-        raise ValueError(f"rope_axes: {names[0]} and {names[1]} must be [M, heads * head_dim]")
+        raise ValueError(f"rope_axes: {nx} and {nout} must be [M, heads * head_dim]")
     if pairs < 8 or pairs % 8 or pairs > 128 or 2 * pairs > head_dim or head_dim % 16 or head_dim > 1024:
         raise ValueError("rope_axes: pairs a multiple of 8 up to 128, 2 * pairs <= head_dim, head_dim a multiple of 16 up to 1024")
-    if freqs.numel() != pairs or not freqs.is_contiguous():
+    if freqs.shape[0] != pairs:
         raise ValueError("rope_axes: freqs must hold one value a pair")
     if (pos is None) == (tok_idx is None):
         raise ValueError("rope_axes: exactly one of pos and tok_idx")
     gh = gw = 0
     if pos is not None:
-        _chk(pos, I32, "pos", 2)
-        if tuple(pos.shape) != (M, len(sections)) or not pos.is_contiguous():
+        _dev_chk(dev, I32, 2, pos=pos)
+        if pos.shape[0] != M or pos.shape[1] != axes or not pos.is_contiguous():
             raise ValueError("rope_axes: pos must be a contiguous [M, axes]")
     else:
-        _chk(tok_idx, I32, "tok_idx")
-        if tok_idx.numel() != M or not tok_idx.is_contiguous() or len(sections) != 3 or grid is None or len(grid) != 3:
+        _dev_chk(dev, I32, tok_idx.dim(), tok_idx=tok_idx)
+        if tok_idx.numel() != M or not tok_idx.is_contiguous() or axes != 3 or grid is None or len(grid) != 3:
             raise ValueError("rope_axes: tok_idx must hold M contiguous ids, with three sections and a grid (T, H, W)")
-        gh, gw = int(grid[1]), int(grid[2])
-    _together(x, out, freqs, pos, tok_idx)
-    if M == 0:
-        return out
-    _rows16(x, names[0]), _rows16(out, names[1])
-    if not (x.data_ptr() == out.data_ptr() and _ld(x) == _ld(out)):
-        _apart([(names[1], out)], [(names[0], x)], "rope_axes")
-    _apart([(names[1], out)], [("freqs", freqs), ("pos", pos), ("tok_idx", tok_idx)], "rope_axes")
-    _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), _p(x), 1 if x.dtype == BF16 else 0, _ld16(x), _p(out), _ld16(out), M, heads,
-         head_dim, _p(freqs), len(sections), (C.c_int * 4)(*sections), _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
+        gh, gw = grid[1], grid[2]
+    if M:
+        _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), x.data_ptr(), 1 if dt is BF16 else 0, _ld16(x), out.data_ptr(), _ld16(out), M,
+             heads, head_dim, freqs.data_ptr(), axes, (C.c_int * 4)(*sections), _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
     return out
-
-
-def _ld16(t):
-    """row pitch of a 2-D tensor; a single row's own stride says nothing"""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def rope_axes_fwd(x, heads, head_dim, sections, freqs, out, pos=None, tok_idx=None, grid=None, interleaved=False):
@@ -603,12 +572,12 @@ def rope_axes_fwd(x, heads, head_dim, sections, freqs, out, pos=None, tok_idx=No
     column range of the packed projection will do) turn by position * frequency, axis a owning sections[a] consecutive pairs; the other
     columns are copied.  Pair i is columns (i, pairs + i), or (2 i, 2 i + 1) with ``interleaved``.  ``freqs``: rope_freqs.  The rows'
     places: ``pos`` i32 [M, axes], or ``tok_idx`` i32 (M token ids >= 0) on the ``grid`` (T, H, W).  ``out`` may be ``x``."""
-    return _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, interleaved, False, ("x", "out"))
+    return _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, interleaved, False, "x", "out")
 
 
 def rope_axes_bwd(dout, heads, head_dim, sections, freqs, dx, pos=None, tok_idx=None, grid=None, interleaved=False):
     """gradient of ``rope_axes_fwd``: dx = dout turned back by the same angles (``dx`` may be ``dout``)"""
-    return _rope_axes(dout, heads, head_dim, sections, freqs, dx, pos, tok_idx, grid, interleaved, True, ("dout", "dx"))
+    return _rope_axes(dout, heads, head_dim, sections, freqs, dx, pos, tok_idx, grid, interleaved, True, "dout", "dx")
 
 
 def diff_attention_fwd_ws(B, Nq, Nk, H, Hkv):
@@ -627,38 +596,46 @@ def diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, norm):
     return int(n)
 
 
-def _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal):
-    _chk(q, BF16, "q", 2), _chk(k, BF16, "k", 2), _chk(v, BF16, "v", 2)
-    if B <= 0 or H <= 0 or Hkv <= 0 or H % Hkv or q.shape[0] % B or k.shape[0] % B:
-        raise ValueError(f"{who}: B rows of clips, H a multiple of Hkv")
-    Nq, Nk = q.shape[0] // B, k.shape[0] // B
-    if Nq == 0 or Nk == 0 or q.shape[1] != H * 128 or k.shape[1] != Hkv * 128 or v.shape != k.shape:
-        raise ValueError(f"{who}: q must be [B * Nq, H * 128], k and v [B * Nk, Hkv * 128]")
-    if lam is None or lam.dtype not in (F32, BF16):
+def _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws):
+    """types and shapes that forward and gradient share -> (device, Nq, Nk)"""
+    for name, t in (("q", q), ("k", k), ("v", v), ("lam", lam)):
+        if t is None or not t.is_cuda:
+            _chk(t, BF16, name)
+    dev = torch.cuda.current_device()
+    pt = lam.dtype
+    if pt is not BF16 and pt is not F32:
         raise TypeError(f"{who}: lam must be f32 or bf16")
-    _chk(lam, lam.dtype, "lam", 3)
-    if lam.shape not in ((4, 1, 64), (4, H, 64)) or not lam.is_contiguous():
+    _dev_chk(dev, BF16, 2, q=q, k=k, v=v)
+    _dev_chk(dev, pt, 3, lam=lam)
+    _dev_chk(dev, pt, 1, gamma=gamma)
+    _dev_chk(dev, I32, 1, kv_len=kv_len)
+    _dev_chk(dev, F32, 1, ws=ws)
+    (Mq, Wq), (Mk, Wk) = q.shape, k.shape
+    if B <= 0 or H <= 0 or Hkv <= 0 or H % Hkv or Mq % B or Mk % B:
+        raise ValueError(f"{who}: B clips of the same number of rows, H a multiple of Hkv")
+    if Mq == 0 or Mk == 0 or Wq != H * 128 or Wk != Hkv * 128 or v.shape != k.shape:
+        raise ValueError(f"{who}: q must be [B * Nq, H * 128], k and v [B * Nk, Hkv * 128]")
+    ls = lam.shape
+    if ls[0] != 4 or ls[1] not in (1, H) or ls[2] != 64 or not lam.is_contiguous():
         raise ValueError(f"{who}: lam must be a contiguous [4, 1 or H, 64]")
-    if gamma is not None:
-        _chk(gamma, lam.dtype, "gamma", 1)
-        if gamma.numel() != 128:
-            raise ValueError(f"{who}: gamma must have 128 entries")
-    if kv_len is not None:
-        _chk(kv_len, I32, "kv_len", 1)
-        if kv_len.numel() != B or not kv_len.is_contiguous():
-            raise ValueError(f"{who}: kv_len must have B entries")
+    if gamma is not None and gamma.shape[0] != 128:
+        raise ValueError(f"{who}: gamma must have 128 entries")
+    if kv_len is not None and kv_len.shape[0] != B:
+        raise ValueError(f"{who}: kv_len must have B entries")
     if causal not in (0, 1, 2):
         raise ValueError(f"{who}: causal must be 0, 1 (from the start) or 2 (towards the end)")
-    _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
-    return Nq, Nk
+    return dev, Mq // B, Mk // B
 
 
-def _diff_saved(who, saved, B, Nq, H):
+def _diff_saved(who, dev, saved, B, Nq, H):
     o, o2, lse2 = saved
-    _chk(o, BF16, "o", 2), _chk(o2, BF16, "o2", 2), _chk(lse2, F32, "lse2")
-    if o.shape != (B * Nq, H * 128) or o2.shape != o.shape or not o.is_contiguous() or not o2.is_contiguous() or lse2.numel() != 2 * B * H * Nq or not lse2.is_contiguous():
+    _dev_chk(dev, BF16, 2, o=o, o2=o2)
+    if lse2 is None or lse2.dtype is not F32 or lse2.get_device() != dev:
+        _chk(lse2, F32, "lse2")
+        raise ValueError(f"{who}: lse2 must be on the current device")
+    if (o is None or o2 is None or o.shape[0] != B * Nq or o.shape[1] != H * 128 or o2.shape != o.shape or not o.is_contiguous() or not o2.is_contiguous()
+            or lse2.numel() != 2 * B * H * Nq or not lse2.is_contiguous()):
         raise ValueError(f"{who}: saved must be (o, o2 bf16 [B * Nq, H * 128], lse2 f32 [2, B, H, Nq]), contiguous")
-    _rows16(o, "o"), _rows16(o2, "o2")
     return o, o2, lse2
 
 
@@ -670,22 +647,16 @@ def diff_attention_fwd(q, k, v, B, H, Hkv, scale, lam, lam_init, out, gamma=None
     or a cache of Nk rows a clip.  ``lam`` [4, 1 or H, 64] (f32 or bf16; ``gamma`` alike): lambda = exp(lam0 . lam1) - exp(lam2 . lam3) + lam_init.
     ``kv_len`` i32 [B]: keys each clip holds; ``causal`` 1: key <= query, 2: the queries are the last Nq of the clip's keys.  A row that sees
     no key gives zeros.  ``saved`` = (o, o2, lse2): kept for ``diff_attention_bwd``.  ``ws``: f32, diff_attention_fwd_ws elements."""
-    Nq, Nk = _diff_chk("diff_attention_fwd", q, k, v, B, H, Hkv, lam, gamma, kv_len, causal)
-    _chk(out, BF16, "out", 2)
-    if out.shape != q.shape:
+    dev, Nq, Nk = _diff_chk("diff_attention_fwd", q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
+    _dev_chk(dev, BF16, 2, out=out)
+    if out is None or out.shape != q.shape:
         raise ValueError("diff_attention_fwd: out must have q's shape")
-    _rows16(out, "out")
-    o, o2, lse2 = (None, None, None) if saved is None else _diff_saved("diff_attention_fwd", saved, B, Nq, H)
-    if ws is not None:
-        _chk(ws, F32, "ws", 1)
-        if not ws.is_contiguous():
-            raise ValueError("diff_attention_fwd: ws must be contiguous")
-    _together(q, k, v, lam, gamma, kv_len, out, o, o2, lse2, ws)
-    _apart([("out", out), ("o", o), ("o2", o2), ("lse2", lse2), ("ws", ws)], [("q", q), ("k", k), ("v", v), ("lam", lam), ("gamma", gamma), ("kv_len", kv_len)],
-           "diff_attention_fwd")
-    _run("mofo_diff_attention_fwd", ("diff_attn_fwd",), 512.0 * B * H * Nq * Nk, _p(q), _ld16(q), _p(k), _ld16(k), _p(v), _ld16(v), B, Nq, Nk, H, Hkv, scale,
-         _p(lam), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype == BF16 else 0, eps, out_scale, _p(kv_len), causal, _p(out), _ld16(out), _p(o), _p(o2),
-         _p(lse2), _p(ws), 0 if ws is None else ws.numel())
+    o = o2 = lse2 = None
+    if saved is not None:
+        o, o2, lse2 = _diff_saved("diff_attention_fwd", dev, saved, B, Nq, H)
+    _run("mofo_diff_attention_fwd", ("diff_attn_fwd",), 512.0 * B * H * Nq * Nk, q.data_ptr(), _ld16(q), k.data_ptr(), _ld16(k), v.data_ptr(), _ld16(v), B, Nq,
+         Nk, H, Hkv, scale, lam.data_ptr(), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype is BF16 else 0, eps, out_scale, _p(kv_len), causal,
+         out.data_ptr(), _ld16(out), _p(o), _p(o2), _p(lse2), _p(ws), 0 if ws is None else ws.numel())
     return out
 
 
@@ -694,32 +665,26 @@ def diff_attention_bwd(q, k, v, B, H, Hkv, scale, lam, lam_init, saved, dout, dq
     """every gradient of ``diff_attention_fwd`` (same arguments, its ``saved``), overwritten: ``dq``, ``dk``, ``dv`` bf16 like q, k, v, ``dlam`` (and
     ``dgamma``) f32 or bf16 like lam (gamma).  ``ws``: f32, diff_attention_bwd_ws elements."""
     who = "diff_attention_bwd"
-    Nq, Nk = _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal)
-    o, o2, lse2 = _diff_saved(who, saved, B, Nq, H)
-    _chk(dout, BF16, "dout", 2), _chk(dq, BF16, "dq", 2), _chk(dk, BF16, "dk", 2), _chk(dv, BF16, "dv", 2), _chk(ws, F32, "ws", 1)
-    if dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
+    dev, Nq, Nk = _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
+    o, o2, lse2 = _diff_saved(who, dev, saved, B, Nq, H)
+    _dev_chk(dev, BF16, 2, dout=dout, dq=dq, dk=dk, dv=dv)
+    if dout is None or dq is None or dk is None or dv is None or dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
         raise ValueError(f"{who}: dout and dq like q, dk and dv like k")
     if dlam is None or dlam.dtype not in (F32, BF16):
         raise TypeError(f"{who}: dlam must be f32 or bf16")
-    _chk(dlam, dlam.dtype, "dlam", 3)
+    gt = dlam.dtype
+    _dev_chk(dev, gt, 3, dlam=dlam)
+    _dev_chk(dev, gt, 1, dgamma=dgamma)
     if dlam.shape != lam.shape or not dlam.is_contiguous():
         raise ValueError(f"{who}: dlam must be contiguous, with lam's shape")
-    if (gamma is None) != (dgamma is None):
-        raise ValueError(f"{who}: gamma and dgamma go together")
-    if dgamma is not None:
-        _chk(dgamma, dlam.dtype, "dgamma", 1)
-        if dgamma.numel() != 128:
-            raise ValueError(f"{who}: dgamma must have 128 entries")
-    for t, n in ((dout, "dout"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
-        _rows16(t, n)
-    if ws.numel() < diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, gamma is not None) or not ws.is_contiguous() or ws.data_ptr() % 16:
-        raise ValueError(f"{who}: ws must hold diff_attention_bwd_ws floats, 16-byte aligned")
-    _together(q, k, v, lam, gamma, kv_len, o, o2, lse2, dout, dq, dk, dv, dlam, dgamma, ws)
-    _apart([("dq", dq), ("dk", dk), ("dv", dv), ("dlam", dlam), ("dgamma", dgamma), ("ws", ws)],
-           [("q", q), ("k", k), ("v", v), ("lam", lam), ("gamma", gamma), ("kv_len", kv_len), ("o", o), ("o2", o2), ("lse2", lse2), ("dout", dout)], who)
-    _run("mofo_diff_attention_bwd", ("diff_attn_bwd",), 1024.0 * B * H * Nq * Nk, _p(q), _ld16(q), _p(k), _ld16(k), _p(v), _ld16(v), B, Nq, Nk, H, Hkv, scale,
-         _p(lam), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype == BF16 else 0, eps, out_scale, _p(kv_len), causal, _p(o), _p(o2), _p(lse2), _p(dout),
-         _ld16(dout), _p(dq), _ld16(dq), _p(dk), _ld16(dk), _p(dv), _ld16(dv), _p(dlam), _p(dgamma), 1 if dlam.dtype == BF16 else 0, _p(ws), ws.numel())
+    if (gamma is None) != (dgamma is None) or (dgamma is not None and dgamma.shape[0] != 128):
+        raise ValueError(f"{who}: gamma and dgamma go together, 128 entries each")
+    if ws is None:
+        raise ValueError(f"{who}: ws must hold diff_attention_bwd_ws floats")
+    _run("mofo_diff_attention_bwd", ("diff_attn_bwd",), 1024.0 * B * H * Nq * Nk, q.data_ptr(), _ld16(q), k.data_ptr(), _ld16(k), v.data_ptr(), _ld16(v), B, Nq,
+         Nk, H, Hkv, scale, lam.data_ptr(), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype is BF16 else 0, eps, out_scale, _p(kv_len), causal,
+         o.data_ptr(), o2.data_ptr(), lse2.data_ptr(), dout.data_ptr(), _ld16(dout), dq.data_ptr(), _ld16(dq), dk.data_ptr(), _ld16(dk), dv.data_ptr(),
+         _ld16(dv), dlam.data_ptr(), _p(dgamma), 1 if gt is BF16 else 0, ws.data_ptr(), ws.numel())
 
 
 def mask_to_indices(mask_u8, n_vis, vis_idx, msk_idx, status):

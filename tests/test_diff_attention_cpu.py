@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-P = 4096     # stands for a 16-byte aligned device pointer
+P = 1 << 20  # stands for a 16-byte aligned device pointer; multiples of it for tensors that lie apart (each call's are smaller than that)
 
 
 def _lib():
@@ -19,7 +19,7 @@ def _error():
 
 
 def _rope(**kw):
-    a = dict(x=P, bf=1, ldx=128, out=2 * P, ldo=128, M=4, heads=2, hd=64, freqs=P, naxes=3, sections=(8, 12, 12, 0), pos=P, tok=None, gh=14, gw=14, inter=0, inv=0)
+    a = dict(x=P, bf=1, ldx=128, out=2 * P, ldo=128, M=4, heads=2, hd=64, freqs=3 * P, naxes=3, sections=(8, 12, 12, 0), pos=4 * P, tok=None, gh=14, gw=14, inter=0, inv=0)
     a.update(kw)
     s = (C.c_int * 4)(*a["sections"]) if a["sections"] is not None else None
     return _lib().mofo_rope_axes(a["x"], a["bf"], a["ldx"], a["out"], a["ldo"], a["M"], a["heads"], a["hd"], a["freqs"], a["naxes"], s, a["pos"], a["tok"], a["gh"],
@@ -30,13 +30,14 @@ def _rope(**kw):
     dict(x=None), dict(out=None), dict(freqs=None), dict(sections=None), dict(M=0), dict(heads=0), dict(hd=0), dict(naxes=0), dict(naxes=5), dict(pos=None),
     dict(tok=P), dict(pos=None, tok=P, naxes=2, sections=(16, 16, 0, 0)), dict(pos=None, tok=P, gw=0), dict(sections=(-8, 20, 20, 0)), dict(sections=(8, 12, 13, 0)),
     dict(sections=(0, 0, 0, 0)), dict(sections=(12, 12, 16, 0)), dict(hd=60), dict(hd=2048, ldx=4096, ldo=4096), dict(ldx=120), dict(ldo=127), dict(ldx=132),
-    dict(x=P + 2), dict(out=2 * P + 8), dict(out=P, ldo=136), dict(bf=0, ldx=130)])
+    dict(x=P + 2), dict(out=2 * P + 8), dict(out=P, ldo=136), dict(bf=0, ldx=130),
+    dict(out=P + 16), dict(out=P + 128, ldx=256, ldo=256), dict(out=3 * P), dict(out=4 * P), dict(pos=None, tok=2 * P + 64)])
 def test_rope_entry_refuses(bad):
     assert _rope(**bad) < 0 and "mofo_rope_axes" in _error()
 
 
 def _fwd(**kw):
-    a = dict(q=P, ldq=512, k=2 * P, ldk=256, v=3 * P, ldv=256, B=2, Nq=5, Nk=7, H=4, Hkv=2, scale=0.125, lam=P, lam_heads=4, lam_init=0.4, gamma=None, pbf=1,
+    a = dict(q=P, ldq=512, k=2 * P, ldk=256, v=3 * P, ldv=256, B=2, Nq=5, Nk=7, H=4, Hkv=2, scale=0.125, lam=5 * P, lam_heads=4, lam_init=0.4, gamma=None, pbf=1,
              eps=1e-5, out_scale=1.0, kv_len=None, causal=0, out=4 * P, ldo=512, o=None, o2=None, lse2=None, ws=None, n=0)
     a.update(kw)
     return _lib().mofo_diff_attention_fwd(*a.values(), None)
@@ -45,23 +46,25 @@ def _fwd(**kw):
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(k=None), dict(v=None), dict(lam=None), dict(out=None), dict(B=0), dict(Nq=0), dict(Nk=-1), dict(H=0), dict(Hkv=0), dict(Hkv=3), dict(scale=0.0),
     dict(scale=-0.5), dict(scale=math.nan), dict(scale=math.inf), dict(lam_heads=2), dict(causal=3), dict(causal=-1), dict(ldq=504), dict(ldk=128), dict(ldv=260),
-    dict(ldk=1 << 25), dict(q=P + 8), dict(k=P + 2), dict(ldo=511), dict(out=P + 4), dict(o=P), dict(o=P, o2=P), dict(lse2=P), dict(o=P + 8, o2=P, lse2=P),
+    dict(ldk=1 << 25), dict(q=P + 8), dict(k=P + 2), dict(ldo=511), dict(out=P + 4), dict(o=6 * P), dict(o=6 * P, o2=7 * P), dict(lse2=8 * P),
+    dict(o=6 * P + 8, o2=7 * P, lse2=8 * P), dict(out=P), dict(out=2 * P), dict(out=P + 1024, ldq=1024, ldo=1032), dict(o=6 * P, o2=6 * P + 64, lse2=8 * P),
+    dict(o=6 * P, o2=7 * P, lse2=4 * P), dict(gamma=4 * P + 16), dict(kv_len=4 * P), dict(Nq=1, Nk=4096, ldk=256, ws=None), dict(Nq=1, Nk=4096, ws=9 * P, n=100),
     dict(H=8192, ldq=1 << 20, ldo=1 << 20, lam_heads=1), dict(B=1 << 20, Nk=1 << 20), dict(Nq=1 << 30)])
 def test_diff_attention_entry_refuses(bad):
     assert _fwd(**bad) < 0 and "mofo_diff_attention_fwd" in _error()
 
 
 def _bwd(**kw):
-    a = dict(q=P, ldq=512, k=2 * P, ldk=256, v=3 * P, ldv=256, B=2, Nq=5, Nk=7, H=4, Hkv=2, scale=0.125, lam=P, lam_heads=4, lam_init=0.4, gamma=None, pbf=1,
-             eps=1e-5, out_scale=1.0, kv_len=None, causal=0, o=P, o2=P, lse2=P, dout=P, lddo=512, dq=P, lddq=512, dk=P, lddk=256, dv=P, lddv=256, dlam=P,
-             dgamma=None, gbf=1, ws=P, n=1 << 30)
+    a = dict(q=P, ldq=512, k=2 * P, ldk=256, v=3 * P, ldv=256, B=2, Nq=5, Nk=7, H=4, Hkv=2, scale=0.125, lam=4 * P, lam_heads=4, lam_init=0.4, gamma=None, pbf=1,
+             eps=1e-5, out_scale=1.0, kv_len=None, causal=0, o=5 * P, o2=6 * P, lse2=7 * P, dout=8 * P, lddo=512, dq=9 * P, lddq=512, dk=10 * P, lddk=256,
+             dv=11 * P, lddv=256, dlam=12 * P, dgamma=None, gbf=1, ws=13 * P, n=1 << 30)
     a.update(kw)
     return _lib().mofo_diff_attention_bwd(*a.values(), None)
 
 
 @pytest.mark.parametrize("bad", [
     dict(o=None), dict(o2=None), dict(lse2=None), dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(dlam=None), dict(ws=None), dict(n=10),
-    dict(gamma=P), dict(dgamma=P), dict(lddo=504), dict(lddq=256), dict(lddk=130), dict(lddv=128), dict(dout=P + 8), dict(ws=P + 4), dict(H=5), dict(q=None)])
+    dict(gamma=20 * P), dict(dgamma=20 * P), dict(dq=P), dict(dk=3 * P), dict(dv=10 * P + 128), dict(dlam=4 * P), dict(ws=8 * P), dict(dq=5 * P), dict(lddo=504), dict(lddq=256), dict(lddk=130), dict(lddv=128), dict(dout=8 * P + 8), dict(ws=13 * P + 4), dict(H=5), dict(q=None)])
 def test_diff_attention_gradient_entry_refuses(bad):
     assert _bwd(**bad) < 0 and "mofo_diff_attention_bwd" in _error()
 
@@ -91,14 +94,3 @@ def test_rope_frequencies():
     want = [1.0, 100.0 ** -0.5, 1.0, 100.0 ** (-1 / 3), 100.0 ** (-2 / 3), 1.0]
     assert f.dtype == torch.float64 and torch.allclose(f * 2 * math.pi, torch.tensor(want, dtype=torch.float64), rtol=1e-15, atol=0)
     assert ops.rope_freqs((0, 8, 0), device="cpu").numel() == 8
-
-
-def test_overlap_of_column_ranges():
-    from mofo_amd import ops
-    buf = torch.zeros(6, 96)
-    assert not ops._overlap(buf[:, :32], buf[:, 32:64]) and not ops._overlap(buf[:, 64:], buf[:, :32])
-    assert ops._overlap(buf[:, :33], buf[:, 32:64]) and ops._overlap(buf, buf[2:3]) and ops._overlap(buf[:3, :32], buf[2:, 16:48])
-    assert not ops._overlap(buf[:3], buf[3:]) and not ops._overlap(buf[:2, 90:], buf[2:, 90:])
-    # the ranges meet in memory when one row's end is the next row's start
-    flat = buf.view(-1)
-    assert ops._overlap(torch.as_strided(flat, (3, 40), (96, 1), 80), torch.as_strided(flat, (3, 40), (96, 1), 10))

@@ -144,8 +144,8 @@ def test_rope_axes_refusals(dev):
             (lambda: ops.rope_axes_fwd(x, 2, 64, (8, 12, 12), f, out, tok_idx=tok), ValueError),
             (lambda: ops.rope_axes_fwd(x, 2, 64, (16, 16), f, out, **ok), ValueError),
             (lambda: ops.rope_axes_fwd(x, 2, 64, (8, 12, 12), f, out, tok_idx=tok[:5], grid=(8, 14, 14)), ValueError),
-            (lambda: ops.rope_axes_fwd(x[:, 1:65], 1, 64, (8, 12, 12), f, out[:, :64], **ok), ValueError),
-            (lambda: ops.rope_axes_fwd(x[:, :64], 1, 64, (8, 12, 12), f, x[:, 16:80], **ok), ValueError),
+            (lambda: ops.rope_axes_fwd(x[:, 1:65], 1, 64, (8, 12, 12), f, out[:, :64], **ok), RuntimeError),
+            (lambda: ops.rope_axes_fwd(x[:, :64], 1, 64, (8, 12, 12), f, x[:, 16:80], **ok), RuntimeError),
             (lambda: ops.rope_axes_fwd(x.cpu(), 2, 64, (8, 12, 12), f, out, **ok), ValueError)]:
         with pytest.raises(err):
             bad()
@@ -562,15 +562,19 @@ def test_diff_attention_refusals(dev):
     for bad in (fwd(q=q.float()), fwd(lam=lam.half()), fwd(gamma=gamma.float()), fwd(kv_len=ln.long()), fwd(out=out.float()), bwd(dlam=lam.half()), bwd(dgamma=gamma.float())):
         with pytest.raises(TypeError):
             bad()
-    for bad in (fwd(B=3), fwd(Hkv=3), fwd(v=v[:8]), fwd(lam=lam[:3]), fwd(lam=lam[:, :3]), fwd(gamma=gamma[:64]), fwd(kv_len=ln[:1]), fwd(causal=3), fwd(out=q),
-                fwd(out=out[:8]), fwd(saved=(saved[0], saved[1], z[:1])), fwd(saved=(saved[0], saved[0], z)), fwd(q=q.cpu()), fwd(saved=(out, saved[1], z)),
-                bwd(dgamma=None), bwd(ws=ws[:-1]), bwd(dq=q), bwd(dk=torch.empty_like(q)), bwd(dout=dout[:8]), bwd(ws=ws[1:])):
+    for bad in (fwd(B=3), fwd(Hkv=3), fwd(v=v[:8]), fwd(lam=lam[:3]), fwd(lam=lam[:, :3]), fwd(gamma=gamma[:64]), fwd(kv_len=ln[:1]), fwd(causal=3),
+                fwd(out=out[:8]), fwd(saved=(saved[0], saved[1], z[:1])), fwd(q=q.cpu()), bwd(dgamma=None), bwd(dk=torch.empty_like(q)), bwd(dout=dout[:8]),
+                bwd(ws=None)):
         with pytest.raises(ValueError):
             bad()
     for bad in (fwd(scale=-1.0), fwd(scale=0.0), fwd(scale=math.nan)):
         with pytest.raises(RuntimeError, match="scale"):
             bad()
+    for bad in (fwd(out=q), fwd(saved=(saved[0], saved[0], z)), fwd(saved=(out, saved[1], z)), bwd(dq=q), bwd(dq=dout)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            bad()
     shifted = torch.empty(B * N, H * 128 + 4, dtype=BF16, device=dev)
-    with pytest.raises(ValueError, match="16 bytes"):
-        fwd(q=shifted[:, 4:])()
+    for bad in (fwd(q=shifted[:, 4:]), bwd(ws=ws[:-1]), bwd(ws=torch.empty(ws.numel() + 1, dtype=F32, device=dev)[1:])):
+        with pytest.raises(RuntimeError):
+            bad()
     fwd()(), bwd()()
