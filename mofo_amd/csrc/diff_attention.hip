@@ -97,30 +97,7 @@ __device__ __forceinline__ Row make_row(const DiffArgs& a, int kvh, int r, int l
     return w;
 }
 
-// staging of a [32 rows][128 + 128 columns] pair of operands into four [32][64] LDS tiles, registers in between; rows at and behind
-// `rows` are zero
-template <int NT>
-struct Stage {
-    static constexpr int PER = 1024 / NT;
-    u32x4 reg[PER];
-    __device__ __forceinline__ void load(const bf16_t* p0, size_t ld0, const bf16_t* p1, size_t ld1, int row0, int rows, int tid) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int idx = tid + NT * j, row = row0 + (idx >> 5), cc = idx & 31;
-            const bf16_t* src = cc < 16 ? p0 + (size_t)row * ld0 + cc * 8 : p1 + (size_t)row * ld1 + (cc - 16) * 8;
-            reg[j] = row < rows ? *(const u32x4*)src : u32x4{0, 0, 0, 0};
-        }
-    }
-    __device__ __forceinline__ void write(unsigned char* buf, int tid) const {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int idx = tid + NT * j, rl = idx >> 5, cc = idx & 31;
-            *(u32x4*)(buf + (cc >> 3) * TILE + rl * RS + (((cc & 7) ^ swz(rl)) << 4)) = reg[j];
-        }
-    }
-};
-
-// LDS-DMA of one operand's [32 rows][64 columns] half tile, as four pieces of 8 rows: rows at and behind `rows` come from a line of zeros
+// LDS-DMA of one operand's [32 rows][64 columns] half tile, as four pieces of 8 rows; rows that are not there come from a line of zeros
 __device__ const u32x4 g_zero = {0, 0, 0, 0};
 struct HalfTile {
     const bf16_t* base;     // first row's 64 columns
@@ -142,8 +119,9 @@ __device__ __forceinline__ void dma_piece(const void* sbase, int voff, unsigned 
                  : "v"(voff), "s"(sbase), "s"(lds_dst)
                  : "memory");
 }
-__device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane) {
-    if (row0 + 32 <= rows) {
+// rows in front of `first` and at and behind `rows` are zero
+__device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane, int first = 0) {
+    if (row0 >= first && row0 + 32 <= rows) {
         const char* p = (const char*)(t.base + (size_t)row0 * t.ld);
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub) dma_piece(p + (size_t)sub * 16 * t.ld, t.voff[sub & 1], lds_dst + sub * 1024);
@@ -151,7 +129,7 @@ __device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int r
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub) {
             const int rl = 8 * sub + (lane >> 3), row = row0 + rl;
-            const void* src = row < rows ? (const void*)(t.base + (size_t)row * t.ld + (((lane & 7) ^ swz(rl)) << 3)) : (const void*)&g_zero;
+            const void* src = row >= first && row < rows ? (const void*)(t.base + (size_t)row * t.ld + (((lane & 7) ^ swz(rl)) << 3)) : (const void*)&g_zero;
             dma_b128(src, lds_dst + sub * 1024);
         }
     }
@@ -522,7 +500,8 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
     }
 }
 
-// block 0 .. lam_heads - 1: the four vectors' gradients of a head (or of all heads); the last block: dgamma
+// block 0 .. lam_heads - 1: the four vectors' gradients of a head (or of all heads); 16 more blocks: 8 columns of dgamma each.  A block's
+// 32 groups of 8 threads walk the partial rows in strides of 32, in a fixed order.
 __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float* __restrict__ part, int nb, void* dlam, void* dgamma, int grad_bf16) {
     __shared__ double red[256];
     const int tid = threadIdx.x;
@@ -530,38 +509,46 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
         if (grad_bf16) ((bf16_t*)p)[i] = f32_to_bf16(v);
         else ((float*)p)[i] = v;
     };
-    if ((int)blockIdx.x < a.lam_heads) {
-        const int h0 = a.lam_heads == 1 ? 0 : blockIdx.x, n = (a.lam_heads == 1 ? a.H : 1) * nb;
-        double s = 0.0;
-        for (int k = tid; k < n; k += 256) s += (double)part[((size_t)h0 * nb + k) * (HV + 1) + HV];
-        red[tid] = s;
+    const bool lam_block = (int)blockIdx.x < a.lam_heads;
+    const int first = lam_block && a.lam_heads > 1 ? blockIdx.x : 0, n = (lam_block && a.lam_heads > 1 ? 1 : a.H) * nb;
+    const int col = lam_block ? HV : 8 * ((int)blockIdx.x - a.lam_heads) + (tid & 7), start = lam_block ? tid : tid >> 3, step = lam_block ? 256 : 32;
+    const float* p = part + (size_t)first * nb * (HV + 1) + col;
+    double s = 0.0;
+    int k = start;
+    for (; k + 7 * step < n; k += 8 * step) {             // eight loads in flight
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[(size_t)(k + e * step) * (HV + 1)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)x[e];
+    }
+    for (; k < n; k += step) s += (double)p[(size_t)k * (HV + 1)];
+    red[tid] = s;
+    __syncthreads();
+    for (int o = 128; o >= (lam_block ? 1 : 8); o >>= 1) {
+        if (tid < o) red[tid] += red[tid + o];
         __syncthreads();
-        for (int o = 128; o > 0; o >>= 1) {
-            if (tid < o) red[tid] += red[tid + o];
-            __syncthreads();
-        }
+    }
+    if (lam_block) {
         const float dl = (float)red[0];
         float e1, e2;
         head_lambda(a, blockIdx.x, tid & 63, e1, e2);
         const int v = tid >> 6;                                    // wave v: vector v; its partner is v ^ 1
         const size_t st = (size_t)a.lam_heads * 64, at = (size_t)blockIdx.x * 64 + (tid & 63);
         put(dlam, v * st + at, dl * (v < 2 ? e1 : -e2) * param(a.lam, a.param_bf16, (v ^ 1) * st + at));
-    } else if (dgamma) {
-        const int d = tid & 127, half = tid >> 7, n = a.H * nb;
-        double s = 0.0;
-        for (int k = half; k < n; k += 2) s += (double)part[(size_t)k * (HV + 1) + d];
-        red[tid] = s;
-        __syncthreads();
-        if (half == 0) put(dgamma, d, (float)(red[d] + red[d + 128]));
+    } else if (tid < 8) {
+        put(dgamma, col, (float)red[tid]);
     }
 }
 
 // dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability, the sign in d_2)
-template <int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                             bf16_t* __restrict__ dq, size_t lddq, int nx) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * 4 * TILE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+// Four waves of 32 rows share the key tiles, ring as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
+__global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                         bf16_t* __restrict__ dq, size_t lddq, int nx) {
+    constexpr int NW = 4, STAGE = 4 * TILE;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
     if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
     const int len = clip_len(a, b);
@@ -570,6 +557,13 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
     int wlo = 0, whi = 0, blo, bhi;
     span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
+    const int nkt = (bhi + 31) >> 5;
+    const size_t kr = (size_t)b * a.Nk;
+    const HalfTile ht = half_tile((wave < 2 ? a.k + kr * a.ldk : a.v + kr * a.ldv) + (size_t)kvh * HV + (wave & 1) * 64, wave < 2 ? a.ldk : a.ldv, lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    auto issue = [&](int t, unsigned buf) { dma_half_tile(ht, t * 32, len, lds0 + buf * STAGE + wave * TILE, lane); };
+    if (nkt > 0) issue(0, 0);
+    if (nkt > 1) issue(1, 1);
     float e1, e2, lam = 0.f;
     const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
     for (int h = h0; h <= h1; ++h) {
@@ -591,18 +585,13 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
     f32x16 dqa[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
-    const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
-    const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
-    const int nkt = (bhi + 31) >> 5;
-    Stage<NW * 64> st;
-    if (nkt > 0) {
-        st.load(kp, a.ldk, vp, a.ldv, 0, len, tid);
-        st.write(smem, tid);
-        __syncthreads();
-    }
+    int buf = 0;
     for (int kt = 0; kt < nkt; ++kt) {
-        const unsigned char* T = smem + (kt & 1) * 4 * TILE;
-        if (kt + 1 < nkt) st.load(kp, a.ldk, vp, a.ldv, (kt + 1) * 32, len, tid);
+        if (kt + 1 < nkt) landed_barrier<4>();
+        else landed_barrier<0>();
+        if (kt + 2 < nkt) issue(kt + 2, buf == 0 ? 2 : buf - 1);
+        const unsigned char* T = smem + buf * STAGE;
+        buf = buf == 2 ? 0 : buf + 1;
         if (kt * 32 < whi) {
             f32x16 g = zero16();
 #pragma unroll
@@ -631,8 +620,6 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
                 }
             }
         }
-        if (kt + 1 < nkt) st.write(smem + ((kt + 1) & 1) * 4 * TILE, tid);
-        __syncthreads();
     }
     if (!w.valid) return;
     const bool some = w.lim > 0;
@@ -647,26 +634,33 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dq_kernel(DiffArgs a, const b
 
 // dK, dV: a wave owns 32 keys and walks the query rows of its key head's G heads.  dV = A^T dO with A = P1 - lam P2,
 // dK_1 = scale dS_1^T Q_1, dK_2 = -lam scale dS_2^T Q_2.  Rows that see nothing are staged as zeros, with a log-sum of 1e30.
-template <int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                              bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
-    constexpr int BUF = 4 * TILE + 512;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * BUF];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5;
+// 128 accumulator registers leave no room for two waves a SIMD with both K and V in registers: V stays in LDS (32 KiB a block), and the
+// dV product comes before G = dO V^T, so that A is gone when G needs its place.  Two LDS stages of Q, dO and the rows' statistics.
+__device__ const f32x4 g_pad_stat = {EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+__global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                          bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
+    constexpr int NW = 4, BUF = 4 * TILE + 512, VAT = 2 * BUF;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[VAT + NW * 2 * TILE];
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
     if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
     const int len = clip_len(a, b);
     const int kb0 = xb * NW * 32, k0 = kb0 + wave * 32, key = k0 + (lane & 31);
-    bf16x8 kf[2][4], vf[8];
-    const size_t krow = (size_t)b * a.Nk + (key < a.Nk ? key : a.Nk - 1);
-    const bf16_t* kp = a.k + krow * a.ldk + (size_t)kvh * HV;
-    const bf16_t* vp = a.v + krow * a.ldv + (size_t)kvh * HV;
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    const unsigned char* Vt = smem + VAT + wave * 2 * TILE;
+    {
+        const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
+        dma_half_tile(half_tile(vp, a.ldv, lane), k0, len, lds0 + VAT + wave * 2 * TILE, lane);
+        dma_half_tile(half_tile(vp + 64, a.ldv, lane), k0, len, lds0 + VAT + wave * 2 * TILE + TILE, lane);
+    }
+    bf16x8 kf[2][4];
+    const bf16_t* kp = a.k + ((size_t)b * a.Nk + (key < a.Nk ? key : a.Nk - 1)) * a.ldk + (size_t)kvh * HV;
     const u32x4 none = {0, 0, 0, 0};
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-        const u32x4 x = key < len ? *(const u32x4*)(kp + 16 * ks + 8 * hh) : none, y = key < len ? *(const u32x4*)(vp + 16 * ks + 8 * hh) : none;
+        const u32x4 x = key < len ? *(const u32x4*)(kp + 16 * ks + 8 * hh) : none;
         kf[ks >> 2][ks & 3] = __builtin_bit_cast(bf16x8, x);
-        vf[ks] = __builtin_bit_cast(bf16x8, y);
     }
     f32x16 dva[4], dka[2][2];
 #pragma unroll
@@ -675,81 +669,94 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dkv_kernel(DiffArgs a, const 
         dka[i >> 1][i & 1] = zero16();
     }
     const int nqt = (a.Nq + 31) >> 5;
-    // query tiles in which some row sees the block's first key: the limits grow with i
+    // the query tiles in which some row sees the block's first key: limits grow with i
     int q_first = 0;
     if (kb0 >= len) q_first = nqt;
     else if (a.causal) {
-        const int need = (a.causal == 1 ? kb0 : kb0 - (len - a.Nq));      // smallest i with lim(i) > kb0
-        q_first = need > 0 ? need >> 5 : 0;
-        if (q_first > nqt) q_first = nqt;
+        const int need = a.causal == 1 ? kb0 : kb0 - (len - a.Nq);       // smallest i with lim(i) > kb0
+        q_first = need > 0 ? min(need >> 5, nqt) : 0;
     }
-    const int per = nqt - q_first, steps = per * a.G;
-    Stage<NW * 64> st;
-    f32x4 sreg = {0, 0, 0, 0};
-    auto load = [&](int t) {
-        const int g = t / per, qt = q_first + (t - g * per), h = kvh * a.G + g;
-        // first row of the clip that sees anything: earlier ones are staged as zeros through `skip`
-        const bf16_t* qp = a.q + (size_t)b * a.Nq * a.ldq + (size_t)h * HV;
-        const bf16_t* op = d_o + (size_t)b * a.Nq * lddo + (size_t)h * HV;
-        st.load(qp, a.ldq, op, lddo, qt * 32, a.Nq, tid);
-        if (a.causal == 2 && len < a.Nq) {
-#pragma unroll
-            for (int j = 0; j < Stage<NW * 64>::PER; ++j)
-                if (row_lim(a, len, qt * 32 + ((tid + NW * 64 * j) >> 5)) <= 0) st.reg[j] = none;
-        }
-        if (tid < 32) {
-            const int i = qt * 32 + tid;
-            sreg = i < a.Nq ? stats[((size_t)b * a.H + h) * a.Nq + i] : f32x4{EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+    const int row_first = a.causal == 2 && len < a.Nq ? a.Nq - len : 0;   // rows in front of it see nothing
+    const int steps = (nqt - q_first) * a.G;
+    const bf16_t* src = wave < 2 ? a.q + (size_t)b * a.Nq * a.ldq + (wave & 1) * 64 : d_o + (size_t)b * a.Nq * lddo + (wave & 1) * 64;
+    HalfTile ht = half_tile(src, wave < 2 ? a.ldq : lddo, lane);
+    auto issue = [&](int g, int qt, unsigned buf) {
+        const int h = kvh * a.G + g;
+        ht.base = src + (size_t)h * HV;
+        dma_half_tile(ht, qt * 32, a.Nq, lds0 + buf * BUF + wave * TILE, lane, row_first);
+        if (wave == 0 && lane < 32) {
+            const int i = qt * 32 + lane;
+            dma_b128(i < a.Nq ? (const void*)(stats + ((size_t)b * a.H + h) * a.Nq + i) : (const void*)&g_pad_stat, lds0 + buf * BUF + 4 * TILE);
         }
     };
-    auto write = [&](int t) {
-        unsigned char* buf = smem + (t & 1) * BUF;
-        st.write(buf, tid);
-        if (tid < 32) *(f32x4*)(buf + 4 * TILE + tid * 16) = sreg;
+    int g = 0, qt = q_first, ng = 0, nqt_next = q_first;                  // this step's tile, the next one's
+    auto advance = [&](int& gg, int& tt) {
+        if (++tt == nqt) {
+            tt = q_first;
+            ++gg;
+        }
     };
-    if (steps > 0) {
-        load(0);
-        write(0);
-        __syncthreads();
-    }
-    int cur_g = -1;
     float sgn = 1.f;
+    if (steps > 0) {
+        issue(0, q_first, 0);
+        advance(ng, nqt_next);
+    } else {
+        landed_barrier<0>();                                              // V's pieces must not outlive the block
+    }
     for (int t = 0; t < steps; ++t) {
-        const int g = t / per, qt = q_first + (t - g * per);
-        if (t + 1 < steps) load(t + 1);
-        if (g != cur_g) {
+        landed_barrier<0>();
+        if (t + 1 < steps) issue(ng, nqt_next, (t + 1) & 1);
+        if (qt == q_first) {                                              // a head begins
             float e1, e2;
             sgn = head_lambda(a, kvh * a.G + g, lane, e1, e2) < 0.f ? -1.f : 1.f;
-            cur_g = g;
         }
         const unsigned char* T = smem + (t & 1) * BUF;
         const f32x4* S = (const f32x4*)(T + 4 * TILE);
-        const int ilast = min(qt * 32 + 31, a.Nq - 1);
-        if (row_lim(a, len, ilast) > k0) {
+        if (row_lim(a, len, min(qt * 32 + 31, a.Nq - 1)) > k0) {
             const bool masked = row_lim(a, len, qt * 32) < k0 + 32;
-            f32x16 gr = zero16();
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) gr = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), vf[ks], gr);
             f32x16 s1 = zero16(), s2 = zero16();
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) s1 = mfma(row_frag(T, ks, lane), kf[0][ks], s1);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) s2 = mfma(row_frag(T + TILE, ks, lane), kf[1][ks], s2);
-            float p1[16], p2[16], A[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const f32x4 rs = S[acc_row(r, hh)];
-                float x1 = fast_exp2(fmaf(s1[r], a.c, -rs[0])), x2 = fast_exp2(fmaf(s2[r], a.c, -rs[1]));
-                if (masked && key >= row_lim(a, len, qt * 32 + acc_row(r, hh))) x1 = x2 = 0.f;
-                A[r] = fmaf(-sgn, x2, x1);
-                p1[r] = x1 * (gr[r] - rs[2]);
-                p2[r] = x2 * fmaf(sgn, gr[r], -rs[3]);
+                s1[r] = fast_exp2(fmaf(s1[r], a.c, -rs[0]));
+                s2[r] = fast_exp2(fmaf(s2[r], a.c, -rs[1]));
+            }
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key >= row_lim(a, len, qt * 32 + acc_row(r, hh))) s1[r] = s2[r] = 0.f;
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const bf16x8 fa = pack_frag(A, s), f1 = pack_frag(p1, s), f2 = pack_frag(p2, s);
+                float A[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) A[r] = fmaf(-sgn, s2[8 * s + r], s1[8 * s + r]);
+                const bf16x8 fa = pack_frag(A, 0);
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt) dva[dt] = mfma(tr_frag(T + (2 + (dt >> 1)) * TILE, s, dt & 1, lane), fa, dva[dt]);
+            }
+            f32x16 gr = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) gr = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), row_frag(Vt + (ks >> 2) * TILE, ks & 3, lane), gr);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const f32x4 rs = S[acc_row(r, hh)];
+                s1[r] *= gr[r] - rs[2];
+                s2[r] *= fmaf(sgn, gr[r], -rs[3]);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                float p1[8], p2[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    p1[r] = s1[8 * s + r];
+                    p2[r] = s2[8 * s + r];
+                }
+                const bf16x8 f1 = pack_frag(p1, 0), f2 = pack_frag(p2, 0);
 #pragma unroll
                 for (int dt = 0; dt < 2; ++dt) {
                     dka[0][dt] = mfma(tr_frag(T, s, dt, lane), f1, dka[0][dt]);
@@ -757,8 +764,8 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_dkv_kernel(DiffArgs a, const 
                 }
             }
         }
-        if (t + 1 < steps) write(t + 1);
-        __syncthreads();
+        advance(g, qt);
+        advance(ng, nqt_next);
     }
     if (key >= a.Nk) return;
     const size_t at = (size_t)b * a.Nk + key;
@@ -819,7 +826,6 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
     return a;
 }
 
-constexpr int FWD_NW = 4;
 unsigned blocks_of(int groups, int nx) { return (unsigned)(8 * ceil_div(groups, 8) * nx); }
 // Waves per block and split of the keys.  Few rows: one block a 32- or 64-row list.  Fewer blocks than the card holds (two of 128 rows a
 // compute unit, three of 32): the keys of each are cut into ranges of at least two tiles, as many as fill it; at most 64 ranges, and
@@ -948,13 +954,13 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
-    const int nx = ceil_div(a.R, 32 * FWD_NW), nk = ceil_div(Nk, 32 * FWD_NW);
-    hipLaunchKernelGGL((diff_dq_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nx)), dim3(FWD_NW * 64), 0, s, a, dy, lddy, stats, (bf16_t*)dq, (size_t)lddq, nx);
+    const int nx = ceil_div(a.R, 128), nk = ceil_div(Nk, 128);
+    hipLaunchKernelGGL(diff_dq_kernel, dim3(blocks_of(B * Hkv, nx)), dim3(256), 0, s, a, dy, lddy, stats, (bf16_t*)dq, (size_t)lddq, nx);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dq)");
-    hipLaunchKernelGGL((diff_dkv_kernel<FWD_NW>), dim3(blocks_of(B * Hkv, nk)), dim3(FWD_NW * 64), 0, s, a, dy, lddy, stats, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
+    hipLaunchKernelGGL(diff_dkv_kernel, dim3(blocks_of(B * Hkv, nk)), dim3(256), 0, s, a, dy, lddy, stats, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
                        (size_t)lddv, nk);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dkv)");
-    hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + 1), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
+    hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + (dgamma ? 16 : 0)), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(params)");
     return MOFO_OK;
 }
