@@ -45,11 +45,9 @@ __device__ __forceinline__ int clip_len(const DiffArgs& a, int b) {
     const int n = a.kv_len[b];
     return n < 0 ? 0 : n > a.Nk ? a.Nk : n;
 }
-__device__ __forceinline__ int row_lim(const DiffArgs& a, int len, int i) {
-    if (a.causal == 0) return len;
-    const int last = (a.causal == 1 ? i : len - a.Nq + i) + 1;
-    return last < 0 ? 0 : last < len ? last : len;
-}
+// causal masks: row i sees the first i + past(len) keys at most
+__device__ __forceinline__ int past(const DiffArgs& a, int len) { return a.causal == 0 ? 1 << 30 : a.causal == 1 ? 1 : len - a.Nq + 1; }
+__device__ __forceinline__ int row_lim(const DiffArgs& a, int len, int i) { return max(0, min(len, i + past(a, len))); }
 // smallest and largest limit of the rows ra .. rb (inclusive) of the list: monotone within a head
 __device__ __forceinline__ void span_lim(const DiffArgs& a, int len, int ra, int rb, int& lo, int& hi) {
     if (a.causal == 0) {
@@ -78,6 +76,46 @@ __device__ __forceinline__ float head_lambda(const DiffArgs& a, int h, int lane,
 }
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
+
+// A lane's byte offsets into a [32][64] half tile, LDS base included (the base a multiple of 128): k step ks of the rows is row ^ 32 ks, columns
+// 32 dt .. 32 dt + 31 are tr ^ 64 dt (first and second four rows of a k step); everything else about a fragment's address is a constant.
+// RowOff / ColOff are made where a phase of a tile begins: kept through a tile loop they would be eight registers.
+#define LDS_AS __attribute__((address_space(3)))
+struct FragOff {
+    unsigned row, tr0, tr1;
+};
+__device__ __forceinline__ FragOff frag_off(unsigned lds, int lane) {
+    const int r = lane & 31, hh = lane >> 5, gg = lane >> 4, i = lane & 15, q = i >> 2, pp = i & 3, ra = 4 * hh + q, rb = ra + 8;
+    const int chunk = 2 * (gg & 1) + (pp >> 1), sub = (pp & 1) * 8;
+    return {lds + r * RS + ((hh ^ swz(r)) << 4), lds + ra * RS + ((chunk ^ swz(ra)) << 4) + sub, lds + rb * RS + ((chunk ^ swz(rb)) << 4) + sub};
+}
+struct RowOff {
+    unsigned o[4];
+    __device__ __forceinline__ RowOff(const FragOff& f) {
+        unsigned x = f.row;
+        asm volatile("" : "+v"(x));
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) o[ks] = x ^ (32 * ks);
+    }
+    __device__ __forceinline__ bf16x8 get(unsigned tile, int ks) const { return *(const LDS_AS bf16x8*)(size_t)(o[ks] + tile); }     // as row_frag
+};
+struct ColOff {
+    unsigned o[2][2];
+    __device__ __forceinline__ ColOff(const FragOff& f) {
+        unsigned x = f.tr0, y = f.tr1;
+        asm volatile("" : "+v"(x), "+v"(y));
+        o[0][0] = x;
+        o[0][1] = y;
+        o[1][0] = x ^ 64;
+        o[1][1] = y ^ 64;
+    }
+    __device__ __forceinline__ bf16x8 get(unsigned tile, int s2, int dt) const {                                                       // as tr_frag
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(size_t)(o[dt][0] + tile + 16 * RS * s2));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(size_t)(o[dt][1] + tile + 16 * RS * s2));
+        const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+        return __builtin_bit_cast(bf16x8, u32x4{l2[0], l2[1], h2[0], h2[1]});
+    }
+};
 
 // one lane's row of a wave tile
 struct Row {
@@ -126,6 +164,7 @@ __device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int r
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub) dma_piece(p + (size_t)sub * 16 * t.ld, t.voff[sub & 1], lds_dst + sub * 1024);
     } else {
+        asm volatile("" : "+v"(lane));     // nothing of this path is to be kept in registers across a tile loop
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub) {
             const int rl = 8 * sub + (lane >> 3), row = row0 + rl;
@@ -416,16 +455,18 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
 // Row pass: dO from dY through the norm, the four numbers per row that the two big passes need, and the parameters' gradients.
 //   g = out_scale * gamma * dY, xhat = O / rms, dO = (g - xhat * mean(g xhat)) / rms;  dgamma += out_scale * dY * xhat
 //   d1 = dO . O1, d2 = dO . O2 (O1 = O + lam O2);  dlam -= d2
-// stats[b, h, i] = (lse_1, lse_2 - log2|lam|, d1, sign(lam) d2): the second map's probability comes out of exp2 already times |lam|.
+// stats[b, h, i] = (-lse_1 / c, -(lse_2 - log2|lam|) / c, -d1, d1 - d2), c = scale log2(e): what the score and G accumulators start from, so that
+// P1 = exp2(c acc), |lam| P2 = exp2(c acc) and G - d1, G - d2 come out of the matrix instructions.
 // 16 lanes a row, a block's rows all of one head; block partials of dgamma / dlam, summed in order by diff_param_kernel.
 __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t* __restrict__ o, const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dout,
                                                         size_t lddo, const float* __restrict__ lse2, bf16_t* __restrict__ d_o, f32x4* __restrict__ stats,
-                                                        float* __restrict__ part) {
+                                                        float* __restrict__ part, float* __restrict__ lams) {
     __shared__ float red[16][HV + 1];
     const int tid = threadIdx.x, lane = tid & 63, sub = tid & 15, slot = tid >> 4, h = blockIdx.y, nb = gridDim.x;
     float e1, e2;
     const float lam = head_lambda(a, h, lane, e1, e2);
-    const float loglam = fast_log2(fabsf(lam)), sgn = lam < 0.f ? -1.f : 1.f;
+    if (blockIdx.x == 0 && tid == 0) lams[h] = lam;
+    const float loglam = fmaxf(fast_log2(fabsf(lam)), -EMPTY_LSE), ic = 1.0f / a.c;    // lam = 0: |lam| P2 = exp2(-1e30) = 0
     float gam[8], dg[8], dl = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -485,7 +526,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
             d1 += __shfl_xor(d1, x, 64);
             d2 += __shfl_xor(d2, x, 64);
         }
-        if (sub == 0) stats[st] = some ? f32x4{lse2[st], lse2[plane + st] - loglam, d1, sgn * d2} : f32x4{EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+        if (sub == 0) stats[st] = some ? f32x4{-lse2[st] * ic, (loglam - lse2[plane + st]) * ic, -d1, d1 - d2} : f32x4{-EMPTY_LSE * ic, -EMPTY_LSE * ic, 0.f, 0.f};
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) red[slot][8 * sub + e] = dg[e];
@@ -541,10 +582,10 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
     }
 }
 
-// dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability, the sign in d_2)
+// dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability)
 // Four waves of 32 rows share the key tiles, ring as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
 __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                         bf16_t* __restrict__ dq, size_t lddq, int nx) {
+                                                         const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx) {
     constexpr int NW = 4, STAGE = 4 * TILE;
     __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
@@ -564,14 +605,6 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
     auto issue = [&](int t, unsigned buf) { dma_half_tile(ht, t * 32, len, lds0 + buf * STAGE + wave * TILE, lane); };
     if (nkt > 0) issue(0, 0);
     if (nkt > 1) issue(1, 1);
-    float e1, e2, lam = 0.f;
-    const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
-    for (int h = h0; h <= h1; ++h) {
-        const float t = head_lambda(a, h, lane, e1, e2);
-        if (w.h == h) lam = t;
-    }
-    const float sgn = lam < 0.f ? -1.f : 1.f;
-
     bf16x8 qf[2][4], of[8];
     const bf16_t* qp = a.q + row_at(a, b, w) * a.ldq + (size_t)w.h * HV;
     const bf16_t* op = d_o + row_at(a, b, w) * lddo + (size_t)w.h * HV;
@@ -582,6 +615,7 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) of[ks] = *(const bf16x8*)(op + 16 * ks + 8 * hh);
     const f32x4 rs = stats[stat_at(a, b, w)];
+    const float nl[2] = {rs[0] * a.c, rs[1] * a.c}, nd[2] = {rs[2], rs[2] + rs[3]};
     f32x16 dqa[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
@@ -603,10 +637,7 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
                 for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
                 float p[16];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float pr = fast_exp2(fmaf(s[r], a.c, -rs[m]));
-                    p[r] = pr * (m == 0 ? g[r] - rs[2] : fmaf(sgn, g[r], -rs[3]));
-                }
+                for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[r], a.c, nl[m])) * (g[r] + nd[m]);
                 if (kt * 32 + 32 > wlo) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
@@ -629,26 +660,46 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
     }
     bf16_t* y = dq + row_at(a, b, w) * lddq + (size_t)w.h * HV;
     store_T(y, dqa[0][0], dqa[0][1], a.scale, hh);
-    store_T(y + 64, dqa[1][0], dqa[1][1], -a.scale, hh);
+    store_T(y + 64, dqa[1][0], dqa[1][1], lams[w.h] < 0.f ? a.scale : -a.scale, hh);
 }
 
 // dK, dV: a wave owns 32 keys and walks the query rows of its key head's G heads.  dV = A^T dO with A = P1 - lam P2,
 // dK_1 = scale dS_1^T Q_1, dK_2 = -lam scale dS_2^T Q_2.  Rows that see nothing are staged as zeros, with a log-sum of 1e30.
 // 128 accumulator registers leave no room for two waves a SIMD with both K and V in registers: V stays in LDS (32 KiB a block), and the
 // dV product comes before G = dO V^T, so that A is gone when G needs its place.  Two LDS stages of Q, dO and the rows' statistics.
-__device__ const f32x4 g_pad_stat = {EMPTY_LSE, EMPTY_LSE, 0.f, 0.f};
+// A row's statistics are wanted by every lane of an accumulator row: each lane splits its own row's numbers into three bf16 terms (exact to
+// f32) and one more matrix instruction, against a selector of ones, spreads a number over the accumulator.  Reading them from LDS per
+// accumulator row cost as much LDS time as two operands.
+__device__ const f32x4 g_pad_stat = {-1.0e36f, -1.0e36f, 0.f, 0.f};     // a row behind the last: exp2(c acc) = 0
+__device__ __forceinline__ bf16x8 split3(float x, float y) {
+    u32x4 f = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+        const uint32_t w = pack_bf16x2(x, y);
+        f[e] = w;
+        x -= bf16lo_to_f32(w);
+        y -= bf16hi_to_f32(w);
+    }
+    return __builtin_bit_cast(bf16x8, f);
+}
+__device__ __forceinline__ bf16x8 selector(uint32_t w) {
+    asm volatile("" : "+v"(w));                                           // made anew where it is used: four hoisted ones are 16 registers
+    return __builtin_bit_cast(bf16x8, u32x4{w, w, w, w});
+}
+
 __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                          bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
+                                                          const float* __restrict__ lams, bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
     constexpr int NW = 4, BUF = 4 * TILE + 512, VAT = 2 * BUF;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[VAT + NW * 2 * TILE];
+    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + NW * 2 * TILE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
     if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
-    const int len = clip_len(a, b);
+    const int len = clip_len(a, b), off = past(a, len);
     const int kb0 = xb * NW * 32, k0 = kb0 + wave * 32, key = k0 + (lane & 31);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
-    const unsigned char* Vt = smem + VAT + wave * 2 * TILE;
+    const FragOff fo = frag_off(lds0, lane);
+    const unsigned vt = VAT + wave * 2 * TILE;
     {
         const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
         dma_half_tile(half_tile(vp, a.ldv, lane), k0, len, lds0 + VAT + wave * 2 * TILE, lane);
@@ -656,10 +707,11 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
     }
     bf16x8 kf[2][4];
     const bf16_t* kp = a.k + ((size_t)b * a.Nk + (key < a.Nk ? key : a.Nk - 1)) * a.ldk + (size_t)kvh * HV;
-    const u32x4 none = {0, 0, 0, 0};
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
-        const u32x4 x = key < len ? *(const u32x4*)(kp + 16 * ks + 8 * hh) : none;
+        u32x4 x = *(const u32x4*)(kp + 16 * ks + 8 * hh);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = key < len ? x[e] : 0u;         // whatever a row behind the clip's last one holds
         kf[ks >> 2][ks & 3] = __builtin_bit_cast(bf16x8, x);
     }
     f32x16 dva[4], dka[2][2];
@@ -670,13 +722,8 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
     }
     const int nqt = (a.Nq + 31) >> 5;
     // the query tiles in which some row sees the block's first key: limits grow with i
-    int q_first = 0;
-    if (kb0 >= len) q_first = nqt;
-    else if (a.causal) {
-        const int need = a.causal == 1 ? kb0 : kb0 - (len - a.Nq);       // smallest i with lim(i) > kb0
-        q_first = need > 0 ? min(need >> 5, nqt) : 0;
-    }
-    const int row_first = a.causal == 2 && len < a.Nq ? a.Nq - len : 0;   // rows in front of it see nothing
+    const int q_first = kb0 >= len ? nqt : min(max(kb0 - off + 1, 0) >> 5, nqt);
+    const int row_first = min(max(1 - off, 0), a.Nq);                     // rows in front of it see nothing
     const int steps = (nqt - q_first) * a.G;
     const bf16_t* src = wave < 2 ? a.q + (size_t)b * a.Nq * a.ldq + (wave & 1) * 64 : d_o + (size_t)b * a.Nq * lddo + (wave & 1) * 64;
     HalfTile ht = half_tile(src, wave < 2 ? a.ldq : lddo, lane);
@@ -684,8 +731,10 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
         const int h = kvh * a.G + g;
         ht.base = src + (size_t)h * HV;
         dma_half_tile(ht, qt * 32, a.Nq, lds0 + buf * BUF + wave * TILE, lane, row_first);
-        if (wave == 0 && lane < 32) {
-            const int i = qt * 32 + lane;
+        int row = lane;
+        asm volatile("" : "+v"(row));
+        if (wave == 0 && row < 32) {
+            const int i = qt * 32 + row;
             dma_b128(i < a.Nq ? (const void*)(stats + ((size_t)b * a.H + h) * a.Nq + i) : (const void*)&g_pad_stat, lds0 + buf * BUF + 4 * TILE);
         }
     };
@@ -703,69 +752,118 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
     } else {
         landed_barrier<0>();                                              // V's pieces must not outlive the block
     }
-    for (int t = 0; t < steps; ++t) {
+    // selectors: the lower half of the lanes offers the score terms, the upper half those of G
+    const uint32_t lower = hh ? 0u : ~0u;
+    auto step = [&](int t, auto buf_tag) {
+        constexpr int PAR = decltype(buf_tag)::value;
         landed_barrier<0>();
-        if (t + 1 < steps) issue(ng, nqt_next, (t + 1) & 1);
-        if (qt == q_first) {                                              // a head begins
-            float e1, e2;
-            sgn = head_lambda(a, kvh * a.G + g, lane, e1, e2) < 0.f ? -1.f : 1.f;
-        }
-        const unsigned char* T = smem + (t & 1) * BUF;
-        const f32x4* S = (const f32x4*)(T + 4 * TILE);
-        if (row_lim(a, len, min(qt * 32 + 31, a.Nq - 1)) > k0) {
-            const bool masked = row_lim(a, len, qt * 32) < k0 + 32;
-            f32x16 s1 = zero16(), s2 = zero16();
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) s1 = mfma(row_frag(T, ks, lane), kf[0][ks], s1);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) s2 = mfma(row_frag(T + TILE, ks, lane), kf[1][ks], s2);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const f32x4 rs = S[acc_row(r, hh)];
-                s1[r] = fast_exp2(fmaf(s1[r], a.c, -rs[0]));
-                s2[r] = fast_exp2(fmaf(s2[r], a.c, -rs[1]));
-            }
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (key >= row_lim(a, len, qt * 32 + acc_row(r, hh))) s1[r] = s2[r] = 0.f;
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float A[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) A[r] = fmaf(-sgn, s2[8 * s + r], s1[8 * s + r]);
-                const bf16x8 fa = pack_frag(A, 0);
-#pragma unroll
-                for (int dt = 0; dt < 4; ++dt) dva[dt] = mfma(tr_frag(T + (2 + (dt >> 1)) * TILE, s, dt & 1, lane), fa, dva[dt]);
-            }
-            f32x16 gr = zero16();
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) gr = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), row_frag(Vt + (ks >> 2) * TILE, ks & 3, lane), gr);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const f32x4 rs = S[acc_row(r, hh)];
-                s1[r] *= gr[r] - rs[2];
-                s2[r] *= fmaf(sgn, gr[r], -rs[3]);
-            }
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float p1[8], p2[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    p1[r] = s1[8 * s + r];
-                    p2[r] = s2[8 * s + r];
-                }
-                const bf16x8 f1 = pack_frag(p1, 0), f2 = pack_frag(p2, 0);
-#pragma unroll
-                for (int dt = 0; dt < 2; ++dt) {
-                    dka[0][dt] = mfma(tr_frag(T, s, dt, lane), f1, dka[0][dt]);
-                    dka[1][dt] = mfma(tr_frag(T + TILE, s, dt, lane), f2, dka[1][dt]);
-                }
-            }
-        }
+        if (t + 1 < steps) issue(ng, nqt_next, 1 - PAR);
+        if (qt == q_first) sgn = lams[kvh * a.G + g] < 0.f ? -1.f : 1.f;  // a head begins
+        constexpr unsigned T = PAR * BUF;
+        const int i0 = qt * 32, last = min(i0 + 31, a.Nq - 1);
         advance(g, qt);
         advance(ng, nqt_next);
+        if (min(len, last + off) > k0) {
+            // four fragment registers: each is refilled right behind the matrix instruction that read it, a group ahead
+            bf16x8 fr[4];
+            RowOff ro(fo);
+            const f32x4 rs = *(const LDS_AS f32x4*)(size_t)(lds0 + T + 4 * TILE + (lane & 31) * 16);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) fr[ks] = ro.get(T, ks);
+            const bf16x8 st = split3(hh ? rs[2] : rs[0], hh ? rs[3] : rs[1]);
+            f32x16 s1 = mfma(st, selector(lower & 0x00003f80u), zero16()), s2 = mfma(st, selector(lower & 0x3f800000u), zero16());
+            
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                s1 = mfma(fr[ks], kf[0][ks], s1);
+                fr[ks] = ro.get(T + TILE, ks);
+                
+            }
+            ColOff co(fo);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                s2 = mfma(fr[ks], kf[1][ks], s2);
+                fr[ks] = co.get(T + (2 + (ks >> 1)) * TILE, 0, ks & 1);
+                
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s1[r] = fast_exp2(s1[r] * a.c);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s2[r] = fast_exp2(s2[r] * a.c);
+            if (min(len, i0 + off) < k0 + 32) {                           // hidden: key >= len or i <= key - off
+                int t = key >= len ? 1 << 30 : key - off - i0 - 4 * hh;
+                asm volatile("" : "+v"(t));
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((r & 3) + 8 * (r >> 2) <= t) s1[r] = s2[r] = 0.f;
+            }
+            
+            {
+                float A[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) A[r] = fmaf(-sgn, s2[r], s1[r]);
+                const bf16x8 fa0 = pack_frag(A, 0), fa1 = pack_frag(A, 1);
+                
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    dva[dt] = mfma(fr[dt], fa0, dva[dt]);
+                    fr[dt] = co.get(T + (2 + (dt >> 1)) * TILE, 1, dt & 1);
+                    
+                }
+                ro = RowOff(fo);
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    dva[dt] = mfma(fr[dt], fa1, dva[dt]);
+                    fr[dt] = (dt & 1) ? ro.get(vt, dt >> 1) : ro.get(T + 2 * TILE, dt >> 1);
+                    
+                }
+            }
+            co = ColOff(fo);
+            f32x16 gr = mfma(st, selector(~lower & 0x00003f80u), zero16());
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                const int x = 2 * (ks & 1), n = ks + 2;
+                gr = mfma(fr[x], fr[x + 1], gr);
+                if (n < 8) {
+                    fr[x] = ro.get(T + (2 + (n >> 2)) * TILE, n & 3);
+                    fr[x + 1] = ro.get(vt + (n >> 2) * TILE, n & 3);
+                } else {
+                    fr[x] = co.get(T, ks & 1, 0);
+                    fr[x + 1] = co.get(T, ks & 1, 1);
+                }
+                
+            }
+            {
+                float p1[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p1[r] = s1[r] * gr[r];
+                const bf16x8 f0 = pack_frag(p1, 0), f1 = pack_frag(p1, 1);
+                gr = mfma(st, selector(~lower & 0x3f800000u), gr);        // G - d1 -> G - d2
+                
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int dt = 0; dt < 2; ++dt) {
+                        dka[0][dt] = mfma(fr[2 * s + dt], s ? f1 : f0, dka[0][dt]);
+                        fr[2 * s + dt] = co.get(T + TILE, s, dt);
+                        
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                float p2[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) p2[r] = s2[8 * s + r] * gr[8 * s + r];
+                u32x4 f2 = __builtin_bit_cast(u32x4, pack_frag(p2, 0));
+                if (sgn < 0.f) f2 ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+                dka[1][0] = mfma(fr[2 * s], __builtin_bit_cast(bf16x8, f2), dka[1][0]);
+                dka[1][1] = mfma(fr[2 * s + 1], __builtin_bit_cast(bf16x8, f2), dka[1][1]);
+            }
+        }
+    };
+    for (int t = 0; t < steps; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>{});
     }
     if (key >= a.Nk) return;
     const size_t at = (size_t)b * a.Nk + key;
@@ -915,7 +1013,7 @@ extern "C" long long mofo_diff_attention_fwd_ws(int B, int Nq, int Nk, int H, in
 extern "C" long long mofo_diff_attention_bwd_ws(int B, int Nq, int Nk, int H, int Hkv, int norm) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd_ws: bad dims");
     const long long rows = (long long)B * Nq * H;
-    return rows * 4 + (norm ? rows * (HV / 2) : 0) + (long long)H * row_blocks(B, Nq, H) * (HV + 1);
+    return rows * 4 + (norm ? rows * (HV / 2) : 0) + (long long)H * row_blocks(B, Nq, H) * (HV + 1) + H;
 }
 
 extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv,
@@ -946,18 +1044,19 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     hipStream_t s = (hipStream_t)stream;
     const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
     const size_t rows = (size_t)B * Nq * H;
-    f32x4* stats = (f32x4*)ws;
+    f32x4* stats = (f32x4*)ws;                            // then dO in bf16 (norm only), block partials, the heads' lambda
     bf16_t* d_o = (bf16_t*)(ws + rows * 4);
     float* part = ws + rows * 4 + (gamma ? rows * (HV / 2) : 0);
+    float* lams = part + (size_t)H * row_blocks(B, Nq, H) * (HV + 1);
     const int nb = row_blocks(B, Nq, H);
-    hipLaunchKernelGGL(diff_rows_kernel, dim3(nb, H), dim3(256), 0, s, a, (const bf16_t*)o, (const bf16_t*)o2, (const bf16_t*)dout, (size_t)lddo, lse2, d_o, stats, part);
+    hipLaunchKernelGGL(diff_rows_kernel, dim3(nb, H), dim3(256), 0, s, a, (const bf16_t*)o, (const bf16_t*)o2, (const bf16_t*)dout, (size_t)lddo, lse2, d_o, stats, part, lams);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
     const int nx = ceil_div(a.R, 128), nk = ceil_div(Nk, 128);
-    hipLaunchKernelGGL(diff_dq_kernel, dim3(blocks_of(B * Hkv, nx)), dim3(256), 0, s, a, dy, lddy, stats, (bf16_t*)dq, (size_t)lddq, nx);
+    hipLaunchKernelGGL(diff_dq_kernel, dim3(blocks_of(B * Hkv, nx)), dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dq)");
-    hipLaunchKernelGGL(diff_dkv_kernel, dim3(blocks_of(B * Hkv, nk)), dim3(256), 0, s, a, dy, lddy, stats, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
+    hipLaunchKernelGGL(diff_dkv_kernel, dim3(blocks_of(B * Hkv, nk)), dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
                        (size_t)lddv, nk);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dkv)");
     hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + (dgamma ? 16 : 0)), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
