@@ -91,8 +91,8 @@ __device__ __forceinline__ FragOff frag_off(unsigned lds, int lane) {
 }
 struct RowOff {
     unsigned o[4];
-    __device__ __forceinline__ RowOff(const FragOff& f) {
-        unsigned x = f.row;
+    __device__ __forceinline__ RowOff(const FragOff& f, unsigned base = 0) {
+        unsigned x = f.row + base;
         asm volatile("" : "+v"(x));
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) o[ks] = x ^ (32 * ks);
@@ -101,8 +101,8 @@ struct RowOff {
 };
 struct ColOff {
     unsigned o[2][2];
-    __device__ __forceinline__ ColOff(const FragOff& f) {
-        unsigned x = f.tr0, y = f.tr1;
+    __device__ __forceinline__ ColOff(const FragOff& f, unsigned base = 0) {
+        unsigned x = f.tr0 + base, y = f.tr1 + base;
         asm volatile("" : "+v"(x), "+v"(y));
         o[0][0] = x;
         o[0][1] = y;
@@ -206,7 +206,7 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 template <int NW, bool SAVE, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit) {
     constexpr int STAGE = 4 * TILE, PIECES = 16 / NW;     // LDS-DMA pieces a wave issues per stage
-    __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE];
+    __shared__ __attribute__((aligned(128))) unsigned char smem[3 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xs, b, kvh;
@@ -255,6 +255,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
         for (int dt = 0; dt < 4; ++dt) o[m][dt] = zero16();
     }
 
+    const FragOff fo = frag_off(lds0, lane);
     const float keep = KEEP_REF / a.c;                    // in score units
     int buf = 0;
     for (int t = 0; t < nkt; ++t) {
@@ -262,28 +263,47 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
         else landed_barrier<0>();
         if (t + 2 < nkt) issue(t + 2, buf == 0 ? 2 : buf - 1);
         const int k0 = (t0 + t) * 32;
-        const unsigned char* T = smem + buf * STAGE;
+        const unsigned T = buf * STAGE;
         buf = buf == 2 ? 0 : buf + 1;
         if (k0 >= whi) continue;                          // no row of this wave sees the tile
-        bf16x8 pf[2][2];
+        // fragment registers are refilled right behind the matrix instruction that read them
+        bf16x8 fr[4];
+        RowOff ro(fo, T);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) fr[ks] = ro.get(0, ks);
+        f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            s[0] = mfma(fr[ks], qf[0][ks], s[0]);
+            fr[ks] = ro.get(TILE, ks);
+        }
+        ColOff co(fo, T);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            s[1] = mfma(fr[ks], qf[1][ks], s[1]);
+            fr[ks] = co.get((2 + (ks >> 1)) * TILE, 0, ks & 1);
+        }
+        if (k0 + 32 > wlo) {
+            int lim = w.lim - k0 - 4 * hh;
+            asm volatile("" : "+v"(lim));
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((r & 3) + 8 * (r >> 2) >= lim) s[0][r] = s[1][r] = -__builtin_inff();
+        }
+        float tm[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            f32x16 s = zero16();
+            tm[m] = s[m][0];
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
-            if (k0 + 32 > wlo) {
+            for (int r = 1; r < 16; ++r) tm[m] = fmaxf(tm[m], s[m][r]);
+        }
+        if (__any(tm[0] > mx[0] + keep || tm[1] > mx[1] + keep)) {            // the first tile (reference -inf) too
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (k0 + acc_row(r, hh) >= w.lim) s[r] = -__builtin_inff();
-            }
-            float tm = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) tm = fmaxf(tm, s[r]);
-            if (__any(tm > mx[m] + keep)) {               // the first tile (reference -inf) too
-                tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-                const float mn = tm > mx[m] + keep ? tm : mx[m];
-                const float alpha = tm > mx[m] + keep ? fast_exp2((mx[m] - mn) * a.c) : 1.f;
-                mx[m] = mn;
+            for (int m = 0; m < 2; ++m) {
+                const float x = fmaxf(tm[m], __shfl_xor(tm[m], 32, 64));
+                const bool up = x > mx[m] + keep;
+                const float alpha = up ? fast_exp2((mx[m] - x) * a.c) : 1.f;
+                mx[m] = up ? x : mx[m];
                 l[m] *= alpha;
                 if constexpr (SAVE) le[m] *= alpha;
 #pragma unroll
@@ -291,27 +311,30 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
             }
-            const float nmc = -mx[m] * a.c;
+        }
+        // two halves of 16 keys: the second half's exponentials stand beside the first half's products
+        const float nmc[2] = {-mx[0] * a.c, -mx[1] * a.c};
 #pragma unroll
-            for (int h8 = 0; h8 < 2; ++h8) {
+        for (int s2 = 0; s2 < 2; ++s2) {
+            bf16x8 pf[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
                 float p[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    p[r] = fast_exp2(fmaf(s[8 * h8 + r], a.c, nmc));
+                    p[r] = fast_exp2(fmaf(s[m][8 * s2 + r], a.c, nmc[m]));
                     if constexpr (SAVE) le[m] += p[r];
                 }
-                pf[m][h8] = pack_frag(p, 0);
-                l[m] = frag_sum(pf[m][h8], l[m]);
+                pf[m] = pack_frag(p, 0);
+                l[m] = frag_sum(pf[m], l[m]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                o[0][dt] = mfma(fr[dt], pf[0], o[0][dt]);
+                o[1][dt] = mfma(fr[dt], pf[1], o[1][dt]);
+                if (s2 == 0) fr[dt] = co.get((2 + (dt >> 1)) * TILE, 1, dt & 1);
             }
         }
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const bf16x8 vf = tr_frag(T + (2 + (dt >> 1)) * TILE, s2, dt & 1, lane);
-                o[0][dt] = mfma(vf, pf[0][s2], o[0][dt]);
-                o[1][dt] = mfma(vf, pf[1][s2], o[1][dt]);
-            }
     }
 
     const bool some = w.lim > t0 * 32 && nkt > 0;          // the row sees a key of this range
@@ -587,7 +610,7 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
 __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
                                                          const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx) {
     constexpr int NW = 4, STAGE = 4 * TILE;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[3 * STAGE];
+    __shared__ __attribute__((aligned(128))) unsigned char smem[3 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
@@ -619,38 +642,62 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
     f32x16 dqa[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
+    const FragOff fo = frag_off(lds0, lane);
     int buf = 0;
     for (int kt = 0; kt < nkt; ++kt) {
         if (kt + 1 < nkt) landed_barrier<4>();
         else landed_barrier<0>();
         if (kt + 2 < nkt) issue(kt + 2, buf == 0 ? 2 : buf - 1);
-        const unsigned char* T = smem + buf * STAGE;
+        const unsigned T = buf * STAGE;
         buf = buf == 2 ? 0 : buf + 1;
-        if (kt * 32 < whi) {
-            f32x16 g = zero16();
+        if (kt * 32 >= whi) continue;
+        bf16x8 fr[4];
+        RowOff ro(fo, T);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) g = mfma(row_frag(T + (2 + (ks >> 2)) * TILE, ks & 3, lane), of[ks], g);
+        for (int ks = 0; ks < 4; ++ks) fr[ks] = ro.get(0, ks);
+        f32x16 s[2] = {zero16(), zero16()}, g = zero16();
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                f32x16 s = zero16();
+        for (int ks = 0; ks < 4; ++ks) {
+            s[0] = mfma(fr[ks], qf[0][ks], s[0]);
+            fr[ks] = ro.get(2 * TILE, ks);
+        }
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = mfma(row_frag(T + m * TILE, ks, lane), qf[m][ks], s);
-                float p[16];
+        for (int ks = 0; ks < 4; ++ks) {
+            g = mfma(fr[ks], of[ks], g);
+            fr[ks] = ro.get(3 * TILE, ks);
+        }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] = fast_exp2(fmaf(s[r], a.c, nl[m])) * (g[r] + nd[m]);
-                if (kt * 32 + 32 > wlo) {
+        for (int ks = 0; ks < 4; ++ks) {
+            g = mfma(fr[ks], of[4 + ks], g);
+            fr[ks] = ro.get(TILE, ks);
+        }
+        ColOff co(fo, T);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (kt * 32 + acc_row(r, hh) >= w.lim) p[r] = 0.f;
-                }
-                const bf16x8 f0 = pack_frag(p, 0), f1 = pack_frag(p, 1);
+        for (int ks = 0; ks < 4; ++ks) {
+            s[1] = mfma(fr[ks], qf[1][ks], s[1]);
+            fr[ks] = co.get(0, ks >> 1, ks & 1);
+        }
+        if (kt * 32 + 32 > wlo) {
+            int lim = w.lim - kt * 32 - 4 * hh;
+            asm volatile("" : "+v"(lim));
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((r & 3) + 8 * (r >> 2) >= lim) s[0][r] = s[1][r] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                float p[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) p[r] = fast_exp2(fmaf(s[m][8 * s2 + r], a.c, nl[m])) * (g[8 * s2 + r] + nd[m]);
+                const bf16x8 f = pack_frag(p, 0);
 #pragma unroll
                 for (int dt = 0; dt < 2; ++dt) {
-                    dqa[m][dt] = mfma(tr_frag(T + m * TILE, 0, dt, lane), f0, dqa[m][dt]);
-                    dqa[m][dt] = mfma(tr_frag(T + m * TILE, 1, dt, lane), f1, dqa[m][dt]);
+                    dqa[m][dt] = mfma(fr[2 * s2 + dt], f, dqa[m][dt]);
+                    if (m == 0) fr[2 * s2 + dt] = co.get(TILE, s2, dt);
                 }
             }
-        }
     }
     if (!w.valid) return;
     const bool some = w.lim > 0;
