@@ -3,8 +3,8 @@
 // A head has TWO softmax maps over 64-wide queries / keys and one 128-wide value (a head row is q1|q2, k1|k2, v: 128 columns each):
 //     S_m = scale * Q_m K_m^T,   P_m = softmax over the row's visible keys,   lam = exp(l0.l1) - exp(l2.l3) + lam_init,
 //     O = (P1 - lam P2) V,       Y = out_scale * gamma * O / sqrt(mean(O^2) + eps)      (Y = O without gamma).
-// Query rows of the G = H / Hkv heads that share a key head are ONE list of R = G * Nq rows (row g * Nq + i): shared key heads cost
-// nothing extra in any pass and their gradients are summed inside a block, in a fixed order.
+// Query rows of the G = H / Hkv heads that share a key head are ONE list of R = G * Nq rows (row i * G + g: limits grow along it): shared key
+// heads cost nothing extra in any pass and their gradients are summed inside a block, in a fixed order.
 // Every mask here is a prefix: row i of clip b sees keys j < lim(b, i), lim = kv_len[b], cut at i + 1 (causal from the start) or at
 // kv_len[b] - Nq + i + 1 (causal towards the end, new tokens behind a cache).  lim = 0: the row's outputs and gradients are zero.
 // Rows of k / v at and behind kv_len[b] are never used: they are replaced by zeros on the way into LDS, whatever they hold.
@@ -48,15 +48,10 @@ __device__ __forceinline__ int clip_len(const DiffArgs& a, int b) {
 // causal masks: row i sees the first i + past(len) keys at most
 __device__ __forceinline__ int past(const DiffArgs& a, int len) { return a.causal == 0 ? 1 << 30 : a.causal == 1 ? 1 : len - a.Nq + 1; }
 __device__ __forceinline__ int row_lim(const DiffArgs& a, int len, int i) { return max(0, min(len, i + past(a, len))); }
-// smallest and largest limit of the rows ra .. rb (inclusive) of the list: monotone within a head
+// smallest and largest limit of the rows ra .. rb (inclusive) of the list
 __device__ __forceinline__ void span_lim(const DiffArgs& a, int len, int ra, int rb, int& lo, int& hi) {
-    if (a.causal == 0) {
-        lo = hi = len;
-        return;
-    }
-    const bool one = a.G == 1 || ra / a.Nq == rb / a.Nq;
-    lo = row_lim(a, len, one ? ra % a.Nq : 0);
-    hi = row_lim(a, len, one ? rb % a.Nq : a.Nq - 1);
+    lo = row_lim(a, len, a.G == 1 ? ra : ra / a.G);
+    hi = row_lim(a, len, a.G == 1 ? rb : rb / a.G);
 }
 __device__ __forceinline__ float param(const void* p, int bf, size_t i) { return bf ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i]; }
 __device__ __forceinline__ f32x4 gamma4(const DiffArgs& a, int d) {
@@ -128,11 +123,40 @@ __device__ __forceinline__ Row make_row(const DiffArgs& a, int kvh, int r, int l
     Row w;
     w.valid = r < a.R;
     if (!w.valid) r = a.R - 1;
-    const int g = a.G == 1 ? 0 : r / a.Nq;
-    w.i = r - g * a.Nq;
-    w.h = kvh * a.G + g;
+    w.i = a.G == 1 ? r : r / a.G;
+    w.h = kvh * a.G + r - w.i * a.G;
     w.lim = w.valid ? row_lim(a, len, w.i) : 0;
     return w;
+}
+
+// A wave's 32 rows of 128 results, held in accumulator layout (row on the lane), leave through its own piece of LDS as whole rows: 16 bytes a
+// lane, 256 bytes a row (straight from the accumulators a store covers 16 bytes of each of 32 rows, 2.1 TB/s).
+constexpr int OUT_ROW = 272, OUT_WAVE = 32 * OUT_ROW;       // rows padded by 16 bytes: no bank conflicts
+__device__ __forceinline__ void out_put(unsigned char* lds, int lane, int dt, int rg, float v0, float v1, float v2, float v3) {
+    *(u32x2*)(lds + (lane & 31) * OUT_ROW + 64 * dt + 16 * rg + 8 * (lane >> 5)) = u32x2{pack_bf16x2(v0, v1), pack_bf16x2(v2, v3)};
+}
+__device__ __forceinline__ void out_put16(unsigned char* lds, int lane, int dt, const f32x16& x, float mul) {
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) out_put(lds, lane, dt, rg, x[4 * rg] * mul, x[4 * rg + 1] * mul, x[4 * rg + 2] * mul, x[4 * rg + 3] * mul);
+}
+// row(r): where row r of the tile goes, or NULL
+template <class F>
+__device__ __forceinline__ void out_flush(const unsigned char* lds, int lane, F row) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int r = 4 * j + (lane >> 4);
+        const u32x4 x = *(const u32x4*)(lds + r * OUT_ROW + (lane & 15) * 16);
+        bf16_t* p = row(r);
+        if (p) *(u32x4*)(p + (lane & 15) * 8) = x;
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+// row r0 + r of the list in a tensor of row pitch ld, columns of its head
+__device__ __forceinline__ bf16_t* list_row(const DiffArgs& a, bf16_t* base, size_t ld, int b, int kvh, int r) {
+    if (r >= a.R) return nullptr;
+    const int i = a.G == 1 ? r : r / a.G;
+    return base + ((size_t)b * a.Nq + i) * ld + (size_t)(kvh * a.G + r - i * a.G) * HV;
 }
 
 // LDS-DMA of one operand's [32 rows][64 columns] half tile, as four pieces of 8 rows; rows that are not there come from a line of zeros
@@ -205,13 +229,16 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // tiles go through a ring of three LDS stages, filled by LDS-DMA two stages ahead, one barrier a tile.
 template <int NW, bool SAVE, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit) {
-    constexpr int STAGE = 4 * TILE, PIECES = 16 / NW;     // LDS-DMA pieces a wave issues per stage
-    __shared__ __attribute__((aligned(128))) unsigned char smem[3 * STAGE];
+    constexpr int STAGE = 4 * TILE, PIECES = 16 / NW;     // LDS-DMA pieces a wave issues per tile
+    constexpr bool PAIR = NW == 4;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[(PAIR ? 4 : 3) * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xs, b, kvh;
     if (!decode_block(nx * nsplit, a.B * a.Hkv, a.Hkv, xs, b, kvh)) return;
-    const int xb = xs / nsplit, sp = xs - xb * nsplit;
+    int xb = xs / nsplit;
+    const int sp = xs - xb * nsplit;
+    if (a.causal) xb = nx - 1 - xb;                       // the longest blocks first
     const int len = clip_len(a, b);
     const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
@@ -219,7 +246,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
     span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
     // this block's range of key tiles
-    const int tiles = (bhi + 31) >> 5, chunk = (tiles + nsplit - 1) / nsplit;
+    const int tiles = (bhi + 31) >> 5, chunk = ((a.Nk + 31) / 32 + nsplit - 1) / nsplit;
     const int t0 = min(sp * chunk, tiles), t1 = min(t0 + chunk, tiles), nkt = t1 - t0;
 
     HalfTile ht[4 / NW > 0 ? 4 / NW : 1];
@@ -259,12 +286,21 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
     const float keep = KEEP_REF / a.c;                    // in score units
     int buf = 0;
     for (int t = 0; t < nkt; ++t) {
-        if (t + 1 < nkt) landed_barrier<PIECES>();
-        else landed_barrier<0>();
-        if (t + 2 < nkt) issue(t + 2, buf == 0 ? 2 : buf - 1);
+        if constexpr (PAIR) {
+            if ((t & 1) == 0) {
+                landed_barrier<0>();
+                if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
+                if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
+            }
+            buf = t & 3;
+        } else {
+            if (t + 1 < nkt) landed_barrier<PIECES>();
+            else landed_barrier<0>();
+            if (t + 2 < nkt) issue(t + 2, buf == 0 ? 2 : buf - 1);
+        }
         const int k0 = (t0 + t) * 32;
         const unsigned T = buf * STAGE;
-        buf = buf == 2 ? 0 : buf + 1;
+        if constexpr (!PAIR) buf = buf == 2 ? 0 : buf + 1;
         if (k0 >= whi) continue;                          // no row of this wave sees the tile
         // fragment registers are refilled right behind the matrix instruction that read them
         bf16x8 fr[4];
@@ -349,6 +385,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
     if constexpr (SPLIT) {
         if (!w.valid) return;
         const size_t pi = stat_at(a, b, w) * nsplit + sp;
+        if (nkt == 0) {                                   // the join does not read a range of weight zero
+            if (hh == 0) f.part_lse[pi * 2] = f.part_lse[pi * 2 + 1] = -__builtin_inff();
+            return;
+        }
         float* pp = f.part + pi * (2 * HV);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -365,12 +405,12 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
         }
     } else {
     float e1, e2, lam = 0.f;
-    const int h0 = kvh * a.G + (a.G == 1 ? 0 : min(r0, a.R - 1) / a.Nq), h1 = kvh * a.G + (a.G == 1 ? 0 : min(r0 + 31, a.R - 1) / a.Nq);
-    for (int h = h0; h <= h1; ++h) {
+    for (int h = kvh * a.G; h < (kvh + 1) * a.G; ++h) {
         const float t = head_lambda(a, h, lane, e1, e2);
         if (w.h == h) lam = t;
     }
-    const size_t col = (size_t)w.h * HV, own = row_at(a, b, w) * a.H * HV + col + 4 * hh;
+    __syncthreads();                                      // the ring is free
+    unsigned char* lds = smem + wave * OUT_WAVE;
     float ss = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
@@ -384,39 +424,39 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
                 ss = fmaf(x[e], x[e], ss);
                 o[0][dt][4 * rg + e] = x[e];
             }
-            if constexpr (SAVE) {
-                if (w.valid) {
-                    *(u32x2*)(f.o + own + 32 * dt + 8 * rg) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-                    *(u32x2*)(f.o2 + own + 32 * dt + 8 * rg) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);            // everything at once does not fit beside the accumulators
+            if constexpr (SAVE) out_put(lds, lane, dt, rg, y[0], y[1], y[2], y[3]);
         }
+        __builtin_amdgcn_sched_barrier(0);                // everything at once does not fit beside the accumulators
     }
-    ss += __shfl_xor(ss, 32, 64);
-    if (!w.valid) return;
     if constexpr (SAVE) {
-        if (hh == 0) {
+        const size_t HW = (size_t)a.H * HV;
+        out_flush(lds, lane, [&](int r) { return list_row(a, f.o2, HW, b, kvh, r0 + r); });
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) out_put16(lds, lane, dt, o[0][dt], 1.f);
+        out_flush(lds, lane, [&](int r) { return list_row(a, f.o, HW, b, kvh, r0 + r); });
+        if (w.valid && hh == 0) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) f.lse2[(size_t)m * a.B * a.H * a.Nq + stat_at(a, b, w)] = some ? lse[m] : EMPTY_LSE;
         }
     }
     if (a.gamma) {
+        ss += __shfl_xor(ss, 32, 64);
         const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) {
 #pragma unroll
             for (int rg = 0; rg < 4; ++rg) {
-                const f32x4 g = gamma4(a, 32 * dt + 8 * rg + 4 * hh);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[0][dt][4 * rg + e] *= rn * g[e];
+                const f32x4 gm = gamma4(a, 32 * dt + 8 * rg + 4 * hh);
+                out_put(lds, lane, dt, rg, o[0][dt][4 * rg] * rn * gm[0], o[0][dt][4 * rg + 1] * rn * gm[1], o[0][dt][4 * rg + 2] * rn * gm[2],
+                        o[0][dt][4 * rg + 3] * rn * gm[3]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+    } else if (!SAVE) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) out_put16(lds, lane, dt, o[0][dt], 1.f);
     }
-    bf16_t* y = f.out + row_at(a, b, w) * f.ldo + col;
-    store_T(y, o[0][0], o[0][1], 1.f, hh);
-    store_T(y + 64, o[0][2], o[0][3], 1.f, hh);
+    out_flush(lds, lane, [&](int r) { return list_row(a, f.out, f.ldo, b, kvh, r0 + r); });
     }
 }
 
@@ -440,12 +480,17 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
     }
     const float* pp = f.part + row * nsplit * (2 * HV) + m * HV + d;
     f32x4 acc = {0, 0, 0, 0};
-    for (int s = 0; s < nsplit; ++s) {
-        const f32x4 x = *(const f32x4*)(pp + (size_t)s * (2 * HV));
-        // lane s holds range s's weight of both maps
-        const float w0 = __shfl(wgt[0], s, 64), w1 = __shfl(wgt[1], s, 64), w = m ? w1 : w0;
+    for (int s0 = 0; s0 < nsplit; s0 += 8) {              // eight loads in flight
+        f32x4 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += w * x[e];
+        for (int j = 0; j < 8; ++j) x[j] = *(const f32x4*)(pp + (size_t)min(s0 + j, nsplit - 1) * (2 * HV));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // lane s holds range s's weight of both maps; ranges behind the last have none
+            const float w0 = __shfl(wgt[0], s0 + j, 64), w1 = __shfl(wgt[1], s0 + j, 64), w = m ? w1 : w0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += w != 0.f ? w * x[j][e] : 0.f;
+        }
     }
     f32x4 o2;
 #pragma unroll
@@ -610,11 +655,12 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
 __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
                                                          const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx) {
     constexpr int NW = 4, STAGE = 4 * TILE;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[3 * STAGE];
+    __shared__ __attribute__((aligned(128))) unsigned char smem[4 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
     if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+    if (a.causal) xb = nx - 1 - xb;                       // the longest blocks first
     const int len = clip_len(a, b);
     const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
@@ -643,13 +689,13 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
     const FragOff fo = frag_off(lds0, lane);
-    int buf = 0;
     for (int kt = 0; kt < nkt; ++kt) {
-        if (kt + 1 < nkt) landed_barrier<4>();
-        else landed_barrier<0>();
-        if (kt + 2 < nkt) issue(kt + 2, buf == 0 ? 2 : buf - 1);
-        const unsigned T = buf * STAGE;
-        buf = buf == 2 ? 0 : buf + 1;
+        if ((kt & 1) == 0) {
+            landed_barrier<0>();
+            if (kt + 2 < nkt) issue(kt + 2, (kt + 2) & 3);
+            if (kt + 3 < nkt) issue(kt + 3, (kt + 3) & 3);
+        }
+        const unsigned T = (kt & 3) * STAGE;
         if (kt * 32 >= whi) continue;
         bf16x8 fr[4];
         RowOff ro(fo, T);
@@ -699,15 +745,20 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
                 }
             }
     }
-    if (!w.valid) return;
     const bool some = w.lim > 0;
-    if (!some) {
+    const float m1 = some ? a.scale : 0.f, m2 = lams[w.h] < 0.f ? m1 : -m1;
+    if (!some) {                                          // not times zero: a row that sees nothing may hold NaN
 #pragma unroll
         for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
     }
-    bf16_t* y = dq + row_at(a, b, w) * lddq + (size_t)w.h * HV;
-    store_T(y, dqa[0][0], dqa[0][1], a.scale, hh);
-    store_T(y + 64, dqa[1][0], dqa[1][1], lams[w.h] < 0.f ? a.scale : -a.scale, hh);
+    __syncthreads();                                      // the ring is free
+    unsigned char* lds = smem + wave * OUT_WAVE;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+        out_put16(lds, lane, dt, dqa[0][dt], m1);
+        out_put16(lds, lane, 2 + dt, dqa[1][dt], m2);
+    }
+    out_flush(lds, lane, [&](int r) { return list_row(a, dq, lddq, b, kvh, r0 + r); });
 }
 
 // dK, dV: a wave owns 32 keys and walks the query rows of its key head's G heads.  dV = A^T dO with A = P1 - lam P2,
@@ -912,14 +963,20 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
         step(t, std::integral_constant<int, 0>{});
         if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>{});
     }
-    if (key >= a.Nk) return;
-    const size_t at = (size_t)b * a.Nk + key;
-    bf16_t* pk = dk + at * lddk + (size_t)kvh * HV;
-    bf16_t* pv = dv + at * lddv + (size_t)kvh * HV;
-    store_T(pk, dka[0][0], dka[0][1], a.scale, hh);
-    store_T(pk + 64, dka[1][0], dka[1][1], -a.scale, hh);
-    store_T(pv, dva[0], dva[1], 1.f, hh);
-    store_T(pv + 64, dva[2], dva[3], 1.f, hh);
+    __syncthreads();                                      // the stages are free
+    unsigned char* lds = smem + wave * OUT_WAVE;
+    int l = lane;
+    asm volatile("" : "+v"(l));                         // nothing of this is kept through the loop
+    const size_t row0 = (size_t)b * a.Nk;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+        out_put16(lds, l, dt, dka[0][dt], a.scale);
+        out_put16(lds, l, 2 + dt, dka[1][dt], -a.scale);
+    }
+    out_flush(lds, l, [&](int r) { return k0 + r < a.Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; });
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) out_put16(lds, l, dt, dva[dt], 1.f);
+    out_flush(lds, l, [&](int r) { return k0 + r < a.Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; });
 }
 
 // ------------------------------------------------------------------------------------------------ host
