@@ -54,19 +54,26 @@ __device__ __forceinline__ void span_lim(const DiffArgs& a, int len, int ra, int
     hi = row_lim(a, len, a.G == 1 ? rb : rb / a.G);
 }
 __device__ __forceinline__ float param(const void* p, int bf, size_t i) { return bf ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i]; }
-__device__ __forceinline__ f32x4 gamma4(const DiffArgs& a, int d) {
-    if (a.param_bf16) {
-        const u32x2 w = *(const u32x2*)((const bf16_t*)a.gamma + d);
-        return f32x4{bf16lo_to_f32(w[0]), bf16hi_to_f32(w[0]), bf16lo_to_f32(w[1]), bf16hi_to_f32(w[1])};
-    }
-    return *(const f32x4*)((const float*)a.gamma + d);
+// sum over the wave, in every lane, by lane permutes inside the vector unit (a shuffle goes through LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum_dpp(float x) {
+    x = dpp_add<0x111, 0xf>(x);      // row_shr 1, 2, 4, 8: lane 15 of every row of 16 holds the row's sum
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);      // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3: lane 63 holds all
+    x = dpp_add<0x143, 0xc>(x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 // lambda of head h, and its two exponentials (every lane of the wave)
 __device__ __forceinline__ float head_lambda(const DiffArgs& a, int h, int lane, float& e1, float& e2) {
     const int hl = a.lam_heads == 1 ? 0 : h;
     const size_t st = (size_t)a.lam_heads * 64, o = (size_t)hl * 64 + lane;
-    e1 = expf(wave_sum(param(a.lam, a.param_bf16, o) * param(a.lam, a.param_bf16, st + o)));
-    e2 = expf(wave_sum(param(a.lam, a.param_bf16, 2 * st + o) * param(a.lam, a.param_bf16, 3 * st + o)));
+    e1 = expf(wave_sum_dpp(param(a.lam, a.param_bf16, o) * param(a.lam, a.param_bf16, st + o)));
+    e2 = expf(wave_sum_dpp(param(a.lam, a.param_bf16, 2 * st + o) * param(a.lam, a.param_bf16, 3 * st + o)));
     return e1 - e2 + a.lam_init;
 }
 
@@ -112,6 +119,33 @@ struct ColOff {
     }
 };
 
+// Blocks are dealt round-robin over the 8 XCDs, each with an L2 of its own.  Mostly: the blocks of one (clip, key head) next to each other,
+// every XCD an eighth of that list, so that K and V are fetched by one XCD or two.  `spread`: over all XCDs, the longest blocks of all
+// heads first -- few heads, causal or of ragged lengths, where eighths of the list would be far from equal.  Causal blocks differ in
+// length along x (long ones at the end: `late`, or at the start): within an eighth long and short ones alternate along the list, and the
+// long ones start first.
+__device__ __forceinline__ bool place_block(const DiffArgs& a, int nx, int spread, bool late, int& x, int& b, int& kvh) {
+    const int groups = a.B * a.Hkv, n = groups * nx, id = blockIdx.x;
+    int g, q;
+    if (spread) {
+        if (id >= n) return false;
+        q = id / groups;
+        g = id - q * groups;
+        x = a.causal && late ? nx - 1 - q : q;
+    } else {
+        const int per = (n + 7) >> 3, lo = (id & 7) * per, have = min(per, n - lo), j = id >> 3;
+        if (j >= have) return false;
+        const int half = (have + 1) >> 1, pos = lo + (!a.causal ? j : j < half ? 2 * j : 2 * (have >> 1) - 1 - 2 * (j - half));
+        g = pos / nx;
+        q = pos - g * nx;
+        x = !a.causal ? q : (q & 1) ? q >> 1 : nx - 1 - (q >> 1);
+        if (a.causal && !late) x = nx - 1 - x;
+    }
+    b = g / a.Hkv;
+    kvh = g - b * a.Hkv;
+    return true;
+}
+
 // one lane's row of a wave tile
 struct Row {
     bool valid;
@@ -141,10 +175,10 @@ __device__ __forceinline__ void out_put16(unsigned char* lds, int lane, int dt, 
 }
 // row(r): where row r of the tile goes, or NULL
 template <class F>
-__device__ __forceinline__ void out_flush(const unsigned char* lds, int lane, F row) {
+__device__ __forceinline__ void out_flush(const unsigned char* lds, int lane, F row, int j0 = 0, int j1 = 8) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = j0; j < j1; ++j) {
         const int r = 4 * j + (lane >> 4);
         const u32x4 x = *(const u32x4*)(lds + r * OUT_ROW + (lane & 15) * 16);
         bf16_t* p = row(r);
@@ -203,6 +237,29 @@ __device__ __forceinline__ void landed_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// KEYS4 blocks (few rows, or few blocks): four waves share 32 rows and deal the key tiles -- or a wave's 32 keys the row tiles -- among
+// themselves.  Every wave has a ring of two tiles of its own and meets the others only at the end, where the four sums are added up
+// through LDS in a fixed order.
+__device__ __forceinline__ void landed_own() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void acc_put(unsigned char* lds, int unit, int lane, const f32x16& x, float mul) {
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg)
+        *(f32x4*)(lds + unit * 4096 + rg * 1024 + lane * 16) = f32x4{x[4 * rg] * mul, x[4 * rg + 1] * mul, x[4 * rg + 2] * mul, x[4 * rg + 3] * mul};
+}
+// sum over the four waves of one accumulator: wave v's unit lies at v * stride + unit * 4096
+__device__ __forceinline__ f32x16 acc_sum(const unsigned char* lds, int stride, int unit, int lane) {
+    f32x16 x;
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+        f32x4 t = *(const f32x4*)(lds + unit * 4096 + rg * 1024 + lane * 16);
+#pragma unroll
+        for (int v = 1; v < 4; ++v) t += *(const f32x4*)(lds + v * stride + unit * 4096 + rg * 1024 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * rg + e] = t[e];
+    }
+    return x;
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 struct FwdOut {
     bf16_t *out, *o, *o2;     // out [B * Nq, ldo]; o, o2 [B * Nq, H * 128] or NULL
@@ -225,45 +282,52 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
     return acc;
 }
 
-// One block: NW waves of 32 rows that share the key tiles of one (clip, key head), or of a range of them (nsplit > 1, few blocks).  The
-// tiles go through a ring of three LDS stages, filled by LDS-DMA two stages ahead, one barrier a tile.
-template <int NW, bool SAVE, bool SPLIT>
-__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit) {
-    constexpr int STAGE = 4 * TILE, PIECES = 16 / NW;     // LDS-DMA pieces a wave issues per tile
-    constexpr bool PAIR = NW == 4;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[(PAIR ? 4 : 3) * STAGE];
+// One block: four waves of 32 rows that share the key tiles of one (clip, key head), two tiles a barrier in a ring of four filled by LDS-DMA;
+// or KEYS4.  nsplit > 1: of a range of the keys, joined by diff_join_kernel.
+template <bool KEYS4, bool SAVE, bool SPLIT>
+__global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
+    constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128, XCH = 8 * STAGE;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[KEYS4 ? XCH + 4096 : 4 * STAGE];
+    __shared__ float gam[HV];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xs, b, kvh;
-    if (!decode_block(nx * nsplit, a.B * a.Hkv, a.Hkv, xs, b, kvh)) return;
-    int xb = xs / nsplit;
-    const int sp = xs - xb * nsplit;
-    if (a.causal) xb = nx - 1 - xb;                       // the longest blocks first
+    if (!place_block(a, nx * nsplit, spread, true, xs, b, kvh)) return;
+    const int xb = xs / nsplit, sp = xs - xb * nsplit;
     const int len = clip_len(a, b);
-    const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
+    const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
-    span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
+    span_lim(a, len, rb0, min(rb0 + ROWS, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
-    // this block's range of key tiles
+    // this block's range of key tiles; KEYS4: the wave's own are t0 + wave, t0 + wave + 4, ...
     const int tiles = (bhi + 31) >> 5, chunk = ((a.Nk + 31) / 32 + nsplit - 1) / nsplit;
-    const int t0 = min(sp * chunk, tiles), t1 = min(t0 + chunk, tiles), nkt = t1 - t0;
+    const int t0 = min(sp * chunk, tiles), t1 = min(t0 + chunk, tiles), all = t1 - t0;
+    const int first = KEYS4 ? t0 + wave : t0, stride = KEYS4 ? 4 : 1, nkt = KEYS4 ? (all - wave + 3) >> 2 : all;
 
-    HalfTile ht[4 / NW > 0 ? 4 / NW : 1];
     const bf16_t* kp = a.k + (size_t)b * a.Nk * a.ldk + (size_t)kvh * HV;
     const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
-#pragma unroll
-    for (int j = 0; j < 4 / NW; ++j) {
-        const int ti = wave * (4 / NW) + j;               // K_1, K_2, V columns 0..63, 64..127
-        ht[j] = half_tile((ti < 2 ? kp : vp) + (ti & 1) * 64, ti < 2 ? a.ldk : a.ldv, lane);
-    }
-    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    HalfTile ht = half_tile((KEYS4 || wave < 2 ? kp : vp) + (KEYS4 ? 0 : (wave & 1) * 64), KEYS4 || wave < 2 ? a.ldk : a.ldv, lane), hv;
+    if constexpr (KEYS4) hv = half_tile(vp, a.ldv, lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * 2 * STAGE : 0;
     auto issue = [&](int t, unsigned buf) {
-#pragma unroll
-        for (int j = 0; j < 4 / NW; ++j) dma_half_tile(ht[j], (t0 + t) * 32, len, lds0 + buf * STAGE + (wave * (4 / NW) + j) * TILE, lane);
+        const int row0 = (first + t * stride) * 32;
+        const unsigned at = lds0 + ring + buf * STAGE;
+        if constexpr (KEYS4) {
+            HalfTile hi = ht;
+            dma_half_tile(hi, row0, len, at, lane);
+            hi.base += 64;
+            dma_half_tile(hi, row0, len, at + TILE, lane);
+            hi = hv;
+            dma_half_tile(hi, row0, len, at + 2 * TILE, lane);
+            hi.base += 64;
+            dma_half_tile(hi, row0, len, at + 3 * TILE, lane);
+        } else {
+            dma_half_tile(ht, row0, len, at + wave * TILE, lane);
+        }
     };
     if (nkt > 0) issue(0, 0);
-    if (nkt > 1) issue(1, 1);
+    if (!KEYS4 && nkt > 1) issue(1, 1);
 
     bf16x8 qf[2][4];
     const bf16_t* qp = a.q + row_at(a, b, w) * a.ldq + (size_t)w.h * HV;
@@ -271,6 +335,17 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) qf[m][ks] = *(const bf16x8*)(qp + 64 * m + 16 * ks + 8 * hh);
+
+    // the epilogue's numbers, while the first tiles are on their way: the heads' lambda, gamma times out_scale
+    float lam = 0.f;
+    if constexpr (!SPLIT) {
+        float e1, e2;
+        for (int h = kvh * a.G; h < (kvh + 1) * a.G; ++h) {
+            const float t = head_lambda(a, h, lane, e1, e2);
+            lam = w.h == h ? t : lam;
+        }
+        if (a.gamma && tid < HV) gam[tid] = a.out_scale * param(a.gamma, a.param_bf16, tid);
+    }
 
     f32x16 o[2][4];
     float mx[2], l[2], le[2];          // reference maximum, sum of the rounded terms, sum of the unrounded terms (SAVE)
@@ -282,25 +357,20 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
         for (int dt = 0; dt < 4; ++dt) o[m][dt] = zero16();
     }
 
-    const FragOff fo = frag_off(lds0, lane);
+    const FragOff fo = frag_off(lds0 + ring, lane);
     const float keep = KEEP_REF / a.c;                    // in score units
-    int buf = 0;
     for (int t = 0; t < nkt; ++t) {
-        if constexpr (PAIR) {
-            if ((t & 1) == 0) {
-                landed_barrier<0>();
-                if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
-                if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
-            }
-            buf = t & 3;
-        } else {
-            if (t + 1 < nkt) landed_barrier<PIECES>();
-            else landed_barrier<0>();
-            if (t + 2 < nkt) issue(t + 2, buf == 0 ? 2 : buf - 1);
+        if constexpr (KEYS4) {
+            landed_own();
+            if (t + 1 < nkt) issue(t + 1, (t + 1) & 1);
+        } else if ((t & 1) == 0) {
+            landed_barrier<0>();
+            if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
+            if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
         }
-        const int k0 = (t0 + t) * 32;
+        const unsigned buf = KEYS4 ? t & 1 : t & 3;
+        const int k0 = (first + t * stride) * 32;
         const unsigned T = buf * STAGE;
-        if constexpr (!PAIR) buf = buf == 2 ? 0 : buf + 1;
         if (k0 >= whi) continue;                          // no row of this wave sees the tile
         // fragment registers are refilled right behind the matrix instruction that read them
         bf16x8 fr[4];
@@ -373,47 +443,98 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
         }
     }
 
-    const bool some = w.lim > t0 * 32 && nkt > 0;          // the row sees a key of this range
-    float inv[2], lse[2];
+    bool some = w.lim > first * 32 && nkt > 0;             // the row sees a key of this wave's
+    float lt[2], lx[2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const float lt = l[m] + __shfl_xor(l[m], 32, 64);
-        const float lx = SAVE ? le[m] + __shfl_xor(le[m], 32, 64) : lt;
-        inv[m] = some ? 1.0f / lt : 0.f;
-        lse[m] = mx[m] * a.c + fast_log2(lx);
+        lt[m] = l[m] + __shfl_xor(l[m], 32, 64);
+        lx[m] = SAVE ? le[m] + __shfl_xor(le[m], 32, 64) : lt[m];
     }
+    float inv[2], lse[2];
+    float* xch = (float*)(smem + XCH);
+    if constexpr (KEYS4) {
+        // the four waves' references and sums, [wave][map][reference, rounded sum, sum][32 rows]; a wave without keys of the row: nothing
+        __syncthreads();
+        if (hh == 0) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float* p = xch + (wave * 2 + m) * 96 + lane;
+                p[0] = some ? mx[m] : -__builtin_inff();
+                p[32] = some ? lt[m] : 0.f;
+                p[64] = some ? lx[m] : 0.f;
+            }
+        }
+        __syncthreads();
+        const bool any = w.lim > t0 * 32 && all > 0;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float top = -__builtin_inff(), st = 0.f, sx = 0.f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float x = xch[(v * 2 + m) * 96 + (lane & 31)];
+                top = x > top ? x : top;
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float* p = xch + (v * 2 + m) * 96 + (lane & 31);
+                const float e = p[32] != 0.f ? fast_exp2((p[0] - top) * a.c) : 0.f;
+                st += e * p[32];
+                sx += e * p[64];
+            }
+            inv[m] = some ? fast_exp2((mx[m] - top) * a.c) / st : 0.f;
+            lse[m] = top * a.c + fast_log2(sx);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                if (!some) o[m][dt] = zero16();           // whatever a row that sees nothing holds
+                acc_put(smem + wave * 2 * STAGE, m * 4 + dt, lane, o[m][dt], inv[m]);
+            }
+        some = any;
+        __syncthreads();
+        // wave w goes on with columns 32 w .. 32 w + 31 of both maps
+        o[0][0] = acc_sum(smem, 2 * STAGE, wave, lane);
+        o[1][0] = acc_sum(smem, 2 * STAGE, 4 + wave, lane);
+        inv[0] = inv[1] = 1.f;
+    } else {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            inv[m] = some ? 1.0f / lt[m] : 0.f;
+            lse[m] = mx[m] * a.c + fast_log2(lx[m]);
+        }
+    }
+    constexpr int ND = KEYS4 ? 1 : 4;                     // column tiles this wave still holds, from dt0 on
+    const int dt0 = KEYS4 ? wave : 0;
     if constexpr (SPLIT) {
         if (!w.valid) return;
         const size_t pi = stat_at(a, b, w) * nsplit + sp;
-        if (nkt == 0) {                                   // the join does not read a range of weight zero
-            if (hh == 0) f.part_lse[pi * 2] = f.part_lse[pi * 2 + 1] = -__builtin_inff();
+        if (all <= 0) {                                   // the join does not read a range of weight zero
+            if (hh == 0 && (!KEYS4 || wave == 0)) f.part_lse[pi * 2] = f.part_lse[pi * 2 + 1] = -__builtin_inff();
             return;
         }
         float* pp = f.part + pi * (2 * HV);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
+            for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
                 for (int rg = 0; rg < 4; ++rg) {
                     f32x4 x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = some ? o[m][dt][4 * rg + e] * inv[m] : 0.f;
-                    *(f32x4*)(pp + m * HV + 32 * dt + 8 * rg + 4 * hh) = x;
+                    *(f32x4*)(pp + m * HV + 32 * (dt0 + dt) + 8 * rg + 4 * hh) = x;
                 }
-            if (hh == 0) f.part_lse[pi * 2 + m] = some ? lse[m] : -__builtin_inff();
+            if (hh == 0 && (!KEYS4 || wave == 0)) f.part_lse[pi * 2 + m] = some ? lse[m] : -__builtin_inff();
         }
     } else {
-    float e1, e2, lam = 0.f;
-    for (int h = kvh * a.G; h < (kvh + 1) * a.G; ++h) {
-        const float t = head_lambda(a, h, lane, e1, e2);
-        if (w.h == h) lam = t;
-    }
-    __syncthreads();                                      // the ring is free
-    unsigned char* lds = smem + wave * OUT_WAVE;
+    __syncthreads();                                      // the ring is free, the sums are read
+    // KEYS4: the waves' columns meet in one tile (per output) and leave it 8 rows a wave
+    unsigned char* lds = smem + (KEYS4 ? 0 : wave * OUT_WAVE);
+    constexpr int NEXT = KEYS4 ? OUT_WAVE : 0;            // o2, o, out: one place after the other, or three
     float ss = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
+    for (int dt = 0; dt < ND; ++dt) {
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
             float x[4], y[4];
@@ -424,39 +545,53 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void diff_fwd_kernel(Diff
                 ss = fmaf(x[e], x[e], ss);
                 o[0][dt][4 * rg + e] = x[e];
             }
-            if constexpr (SAVE) out_put(lds, lane, dt, rg, y[0], y[1], y[2], y[3]);
+            if constexpr (SAVE) out_put(lds, lane, dt0 + dt, rg, y[0], y[1], y[2], y[3]);
         }
         __builtin_amdgcn_sched_barrier(0);                // everything at once does not fit beside the accumulators
     }
+    const size_t HW = (size_t)a.H * HV;
     if constexpr (SAVE) {
-        const size_t HW = (size_t)a.H * HV;
-        out_flush(lds, lane, [&](int r) { return list_row(a, f.o2, HW, b, kvh, r0 + r); });
+        if (!KEYS4) out_flush(lds, lane, [&](int r) { return list_row(a, f.o2, HW, b, kvh, r0 + r); });
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) out_put16(lds, lane, dt, o[0][dt], 1.f);
-        out_flush(lds, lane, [&](int r) { return list_row(a, f.o, HW, b, kvh, r0 + r); });
-        if (w.valid && hh == 0) {
+        for (int dt = 0; dt < ND; ++dt) out_put16(lds + NEXT, lane, dt0 + dt, o[0][dt], 1.f);
+        if (!KEYS4) out_flush(lds, lane, [&](int r) { return list_row(a, f.o, HW, b, kvh, r0 + r); });
+        if (w.valid && hh == 0 && (!KEYS4 || wave == 0)) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) f.lse2[(size_t)m * a.B * a.H * a.Nq + stat_at(a, b, w)] = some ? lse[m] : EMPTY_LSE;
         }
     }
     if (a.gamma) {
         ss += __shfl_xor(ss, 32, 64);
-        const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
+        if constexpr (KEYS4) {
+            if (hh == 0) xch[wave * 32 + lane] = ss;
+            __syncthreads();
+            ss = (xch[lane & 31] + xch[32 + (lane & 31)]) + (xch[64 + (lane & 31)] + xch[96 + (lane & 31)]);
+        }
+        const float rn = 1.0f / sqrtf(ss * (1.f / HV) + a.eps);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
+        for (int dt = 0; dt < ND; ++dt) {
 #pragma unroll
             for (int rg = 0; rg < 4; ++rg) {
-                const f32x4 gm = gamma4(a, 32 * dt + 8 * rg + 4 * hh);
-                out_put(lds, lane, dt, rg, o[0][dt][4 * rg] * rn * gm[0], o[0][dt][4 * rg + 1] * rn * gm[1], o[0][dt][4 * rg + 2] * rn * gm[2],
+                const f32x4 gm = *(const f32x4*)(gam + 32 * (dt0 + dt) + 8 * rg + 4 * hh);
+                out_put(lds + 2 * NEXT, lane, dt0 + dt, rg, o[0][dt][4 * rg] * rn * gm[0], o[0][dt][4 * rg + 1] * rn * gm[1], o[0][dt][4 * rg + 2] * rn * gm[2],
                         o[0][dt][4 * rg + 3] * rn * gm[3]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-    } else if (!SAVE) {
+    } else if (!SAVE || KEYS4) {
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) out_put16(lds, lane, dt, o[0][dt], 1.f);
+        for (int dt = 0; dt < ND; ++dt) out_put16(lds + 2 * NEXT, lane, dt0 + dt, o[0][dt], 1.f);
     }
-    out_flush(lds, lane, [&](int r) { return list_row(a, f.out, f.ldo, b, kvh, r0 + r); });
+    if constexpr (KEYS4) {
+        __syncthreads();
+        if constexpr (SAVE) {
+            out_flush(lds, lane, [&](int r) { return list_row(a, f.o2, HW, b, kvh, r0 + r); }, 2 * wave, 2 * wave + 2);
+            out_flush(lds + NEXT, lane, [&](int r) { return list_row(a, f.o, HW, b, kvh, r0 + r); }, 2 * wave, 2 * wave + 2);
+        }
+        out_flush(lds + 2 * NEXT, lane, [&](int r) { return list_row(a, f.out, f.ldo, b, kvh, r0 + r); }, 2 * wave, 2 * wave + 2);
+    } else {
+        out_flush(lds, lane, [&](int r) { return list_row(a, f.out, f.ldo, b, kvh, r0 + r); });
+    }
     }
 }
 
@@ -651,29 +786,46 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
 }
 
 // dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability)
-// Four waves of 32 rows share the key tiles, ring as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
-__global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                         const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx) {
-    constexpr int NW = 4, STAGE = 4 * TILE;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[4 * STAGE];
+// Blocks and rings as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
+template <bool KEYS4>
+__global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                                    const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx, int spread) {
+    constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[(KEYS4 ? 8 : 4) * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
-    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
-    if (a.causal) xb = nx - 1 - xb;                       // the longest blocks first
+    if (!place_block(a, nx, spread, true, xb, b, kvh)) return;
     const int len = clip_len(a, b);
-    const int rb0 = xb * NW * 32, r0 = rb0 + wave * 32;
+    const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
-    span_lim(a, len, rb0, min(rb0 + NW * 32, a.R) - 1, blo, bhi);
+    span_lim(a, len, rb0, min(rb0 + ROWS, a.R) - 1, blo, bhi);
     if (r0 < a.R) span_lim(a, len, r0, min(r0 + 32, a.R) - 1, wlo, whi);
-    const int nkt = (bhi + 31) >> 5;
+    const int all = (bhi + 31) >> 5, first = KEYS4 ? wave : 0, stride = KEYS4 ? 4 : 1, nkt = KEYS4 ? (all - wave + 3) >> 2 : all;
     const size_t kr = (size_t)b * a.Nk;
-    const HalfTile ht = half_tile((wave < 2 ? a.k + kr * a.ldk : a.v + kr * a.ldv) + (size_t)kvh * HV + (wave & 1) * 64, wave < 2 ? a.ldk : a.ldv, lane);
-    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
-    auto issue = [&](int t, unsigned buf) { dma_half_tile(ht, t * 32, len, lds0 + buf * STAGE + wave * TILE, lane); };
+    const bf16_t *kp = a.k + kr * a.ldk + (size_t)kvh * HV, *vp = a.v + kr * a.ldv + (size_t)kvh * HV;
+    HalfTile ht = half_tile((KEYS4 || wave < 2 ? kp : vp) + (KEYS4 ? 0 : (wave & 1) * 64), KEYS4 || wave < 2 ? a.ldk : a.ldv, lane), hv;
+    if constexpr (KEYS4) hv = half_tile(vp, a.ldv, lane);
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * 2 * STAGE : 0;
+    auto issue = [&](int t, unsigned buf) {
+        const int row0 = (first + t * stride) * 32;
+        const unsigned at = lds0 + ring + buf * STAGE;
+        if constexpr (KEYS4) {
+            HalfTile hi = ht;
+            dma_half_tile(hi, row0, len, at, lane);
+            hi.base += 64;
+            dma_half_tile(hi, row0, len, at + TILE, lane);
+            hi = hv;
+            dma_half_tile(hi, row0, len, at + 2 * TILE, lane);
+            hi.base += 64;
+            dma_half_tile(hi, row0, len, at + 3 * TILE, lane);
+        } else {
+            dma_half_tile(ht, row0, len, at + wave * TILE, lane);
+        }
+    };
     if (nkt > 0) issue(0, 0);
-    if (nkt > 1) issue(1, 1);
+    if (!KEYS4 && nkt > 1) issue(1, 1);
     bf16x8 qf[2][4], of[8];
     const bf16_t* qp = a.q + row_at(a, b, w) * a.ldq + (size_t)w.h * HV;
     const bf16_t* op = d_o + row_at(a, b, w) * lddo + (size_t)w.h * HV;
@@ -688,15 +840,19 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
     f32x16 dqa[2][2];
 #pragma unroll
     for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
-    const FragOff fo = frag_off(lds0, lane);
-    for (int kt = 0; kt < nkt; ++kt) {
-        if ((kt & 1) == 0) {
+    const FragOff fo = frag_off(lds0 + ring, lane);
+    for (int t = 0; t < nkt; ++t) {
+        if constexpr (KEYS4) {
+            landed_own();
+            if (t + 1 < nkt) issue(t + 1, (t + 1) & 1);
+        } else if ((t & 1) == 0) {
             landed_barrier<0>();
-            if (kt + 2 < nkt) issue(kt + 2, (kt + 2) & 3);
-            if (kt + 3 < nkt) issue(kt + 3, (kt + 3) & 3);
+            if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
+            if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
         }
-        const unsigned T = (kt & 3) * STAGE;
-        if (kt * 32 >= whi) continue;
+        const int k0 = (first + t * stride) * 32;
+        const unsigned T = (KEYS4 ? t & 1 : t & 3) * STAGE;
+        if (k0 >= whi) continue;
         bf16x8 fr[4];
         RowOff ro(fo, T);
 #pragma unroll
@@ -723,8 +879,8 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
             s[1] = mfma(fr[ks], qf[1][ks], s[1]);
             fr[ks] = co.get(0, ks >> 1, ks & 1);
         }
-        if (kt * 32 + 32 > wlo) {
-            int lim = w.lim - kt * 32 - 4 * hh;
+        if (k0 + 32 > wlo) {
+            int lim = w.lim - k0 - 4 * hh;
             asm volatile("" : "+v"(lim));
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -752,13 +908,26 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
         for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
     }
     __syncthreads();                                      // the ring is free
-    unsigned char* lds = smem + wave * OUT_WAVE;
+    if constexpr (KEYS4) {
+        unsigned char* mine = smem + wave * STAGE;
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) {
-        out_put16(lds, lane, dt, dqa[0][dt], m1);
-        out_put16(lds, lane, 2 + dt, dqa[1][dt], m2);
+        for (int dt = 0; dt < 2; ++dt) {
+            acc_put(mine, dt, lane, dqa[0][dt], m1);
+            acc_put(mine, 2 + dt, lane, dqa[1][dt], m2);
+        }
+        __syncthreads();
+        out_put16(smem + 4 * STAGE, lane, wave, acc_sum(smem, STAGE, wave, lane), 1.f);
+        __syncthreads();
+        out_flush(smem + 4 * STAGE, lane, [&](int r) { return list_row(a, dq, lddq, b, kvh, r0 + r); }, 2 * wave, 2 * wave + 2);
+    } else {
+        unsigned char* lds = smem + wave * OUT_WAVE;
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+            out_put16(lds, lane, dt, dqa[0][dt], m1);
+            out_put16(lds, lane, 2 + dt, dqa[1][dt], m2);
+        }
+        out_flush(lds, lane, [&](int r) { return list_row(a, dq, lddq, b, kvh, r0 + r); });
     }
-    out_flush(lds, lane, [&](int r) { return list_row(a, dq, lddq, b, kvh, r0 + r); });
 }
 
 // dK, dV: a wave owns 32 keys and walks the query rows of its key head's G heads.  dV = A^T dO with A = P1 - lam P2,
@@ -785,23 +954,27 @@ __device__ __forceinline__ bf16x8 selector(uint32_t w) {
     return __builtin_bit_cast(bf16x8, u32x4{w, w, w, w});
 }
 
-__global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                          const float* __restrict__ lams, bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx) {
-    constexpr int NW = 4, BUF = 4 * TILE + 512, VAT = 2 * BUF;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + NW * 2 * TILE];
+template <bool ROWS4>
+__global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+                                                          const float* __restrict__ lams, bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx,
+                                                          int spread) {
+    constexpr int BUF = 4 * TILE + 512, VAT = (ROWS4 ? 8 : 2) * BUF;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + (ROWS4 ? 1 : 4) * 2 * TILE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
-    if (!decode_block(nx, a.B * a.Hkv, a.Hkv, xb, b, kvh)) return;
+    if (!place_block(a, nx, spread, false, xb, b, kvh)) return;
     const int len = clip_len(a, b), off = past(a, len);
-    const int kb0 = xb * NW * 32, k0 = kb0 + wave * 32, key = k0 + (lane & 31);
+    const int kb0 = xb * (ROWS4 ? 32 : 128), k0 = kb0 + (ROWS4 ? 0 : wave * 32), key = k0 + (lane & 31);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
+    const unsigned ring = ROWS4 ? wave * 2 * BUF : 0, vt = VAT + (ROWS4 ? 0 : wave * 2 * TILE);
     const FragOff fo = frag_off(lds0, lane);
-    const unsigned vt = VAT + wave * 2 * TILE;
     {
         const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
-        dma_half_tile(half_tile(vp, a.ldv, lane), k0, len, lds0 + VAT + wave * 2 * TILE, lane);
-        dma_half_tile(half_tile(vp + 64, a.ldv, lane), k0, len, lds0 + VAT + wave * 2 * TILE + TILE, lane);
+        if (!ROWS4 || wave == 0) {
+            dma_half_tile(half_tile(vp, a.ldv, lane), k0, len, lds0 + vt, lane);
+            dma_half_tile(half_tile(vp + 64, a.ldv, lane), k0, len, lds0 + vt + TILE, lane);
+        }
     }
     bf16x8 kf[2][4];
     const bf16_t* kp = a.k + ((size_t)b * a.Nk + (key < a.Nk ? key : a.Nk - 1)) * a.ldk + (size_t)kvh * HV;
@@ -822,45 +995,72 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
     // the query tiles in which some row sees the block's first key: limits grow with i
     const int q_first = kb0 >= len ? nqt : min(max(kb0 - off + 1, 0) >> 5, nqt);
     const int row_first = min(max(1 - off, 0), a.Nq);                     // rows in front of it see nothing
-    const int steps = (nqt - q_first) * a.G;
-    const bf16_t* src = wave < 2 ? a.q + (size_t)b * a.Nq * a.ldq + (wave & 1) * 64 : d_o + (size_t)b * a.Nq * lddo + (wave & 1) * 64;
-    HalfTile ht = half_tile(src, wave < 2 ? a.ldq : lddo, lane);
+    const int per = nqt - q_first, all = per * a.G, stride = ROWS4 ? 4 : 1, steps = ROWS4 ? (all - wave + 3) >> 2 : all;
+    const bf16_t *qbase = a.q + (size_t)b * a.Nq * a.ldq, *obase = d_o + (size_t)b * a.Nq * lddo;
+    HalfTile ht = half_tile(ROWS4 || wave < 2 ? qbase : obase, ROWS4 || wave < 2 ? a.ldq : lddo, lane), ho;
+    if constexpr (ROWS4) ho = half_tile(obase, lddo, lane);
     auto issue = [&](int g, int qt, unsigned buf) {
         const int h = kvh * a.G + g;
-        ht.base = src + (size_t)h * HV;
-        dma_half_tile(ht, qt * 32, a.Nq, lds0 + buf * BUF + wave * TILE, lane, row_first);
+        const unsigned at = lds0 + ring + buf * BUF;
+        HalfTile hi = ht;
+        hi.base += (size_t)h * HV;
+        if constexpr (ROWS4) {
+            dma_half_tile(hi, qt * 32, a.Nq, at, lane, row_first);
+            hi.base += 64;
+            dma_half_tile(hi, qt * 32, a.Nq, at + TILE, lane, row_first);
+            hi = ho;
+            hi.base += (size_t)h * HV;
+            dma_half_tile(hi, qt * 32, a.Nq, at + 2 * TILE, lane, row_first);
+            hi.base += 64;
+            dma_half_tile(hi, qt * 32, a.Nq, at + 3 * TILE, lane, row_first);
+        } else {
+            hi.base += (wave & 1) * 64;
+            dma_half_tile(hi, qt * 32, a.Nq, at + wave * TILE, lane, row_first);
+        }
         int row = lane;
         asm volatile("" : "+v"(row));
-        if (wave == 0 && row < 32) {
+        if ((ROWS4 || wave == 0) && row < 32) {
             const int i = qt * 32 + row;
-            dma_b128(i < a.Nq ? (const void*)(stats + ((size_t)b * a.H + h) * a.Nq + i) : (const void*)&g_pad_stat, lds0 + buf * BUF + 4 * TILE);
+            dma_b128(i < a.Nq ? (const void*)(stats + ((size_t)b * a.H + h) * a.Nq + i) : (const void*)&g_pad_stat, at + 4 * TILE);
         }
     };
-    int g = 0, qt = q_first, ng = 0, nqt_next = q_first;                  // this step's tile, the next one's
-    auto advance = [&](int& gg, int& tt) {
-        if (++tt == nqt) {
-            tt = q_first;
+    // this step's head and tile, the next one's: all tiles of a head, then the next head's; ROWS4 in strides of four
+    int g = 0, qt = q_first, ng = 0, nqt_next = q_first;
+    auto advance = [&](int& gg, int& tt, int by) {
+        tt += by;
+        while (tt >= nqt && gg < a.G) {
+            tt -= per;
             ++gg;
         }
     };
-    float sgn = 1.f;
-    if (steps > 0) {
-        issue(0, q_first, 0);
-        advance(ng, nqt_next);
-    } else {
-        landed_barrier<0>();                                              // V's pieces must not outlive the block
+    if (ROWS4 && per > 0) {
+        advance(g, qt, wave);
+        ng = g;
+        nqt_next = qt;
     }
+    float sgn = 1.f;
+    int sgn_of = -1;
+    if (steps > 0) {
+        issue(g, qt, 0);
+        advance(ng, nqt_next, stride);
+    }
+    if (ROWS4) landed_barrier<0>();                                       // V is everybody's
+    else if (steps == 0) landed_barrier<0>();                             // V's pieces must not outlive the block
     // selectors: the lower half of the lanes offers the score terms, the upper half those of G
     const uint32_t lower = hh ? 0u : ~0u;
     auto step = [&](int t, auto buf_tag) {
         constexpr int PAR = decltype(buf_tag)::value;
-        landed_barrier<0>();
+        if constexpr (ROWS4) landed_own();
+        else landed_barrier<0>();
         if (t + 1 < steps) issue(ng, nqt_next, 1 - PAR);
-        if (qt == q_first) sgn = lams[kvh * a.G + g] < 0.f ? -1.f : 1.f;  // a head begins
-        constexpr unsigned T = PAR * BUF;
+        if (g != sgn_of) {                                                // a head begins
+            sgn = lams[kvh * a.G + g] < 0.f ? -1.f : 1.f;
+            sgn_of = g;
+        }
+        const unsigned T = ring + PAR * BUF;
         const int i0 = qt * 32, last = min(i0 + 31, a.Nq - 1);
-        advance(g, qt);
-        advance(ng, nqt_next);
+        advance(g, qt, stride);
+        advance(ng, nqt_next, stride);
         if (min(len, last + off) > k0) {
             // four fragment registers: each is refilled right behind the matrix instruction that read it, a group ahead
             bf16x8 fr[4];
@@ -964,19 +1164,40 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
         if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>{});
     }
     __syncthreads();                                      // the stages are free
-    unsigned char* lds = smem + wave * OUT_WAVE;
     int l = lane;
-    asm volatile("" : "+v"(l));                         // nothing of this is kept through the loop
+    asm volatile("" : "+v"(l));                           // nothing of this is kept through the loop
     const size_t row0 = (size_t)b * a.Nk;
+    auto dk_row = [&](int r) { return k0 + r < a.Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; };
+    auto dv_row = [&](int r) { return k0 + r < a.Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; };
+    if constexpr (ROWS4) {
+        unsigned char* mine = smem + wave * 8 * 4096;
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt) {
-        out_put16(lds, l, dt, dka[0][dt], a.scale);
-        out_put16(lds, l, 2 + dt, dka[1][dt], -a.scale);
+        for (int dt = 0; dt < 2; ++dt) {
+            acc_put(mine, dt, l, dka[0][dt], a.scale);
+            acc_put(mine, 2 + dt, l, dka[1][dt], -a.scale);
+        }
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) acc_put(mine, 4 + dt, l, dva[dt], 1.f);
+        __syncthreads();
+        const f32x16 x = acc_sum(smem, 8 * 4096, wave, l), y = acc_sum(smem, 8 * 4096, 4 + wave, l);
+        __syncthreads();
+        out_put16(smem, l, wave, x, 1.f);
+        out_put16(smem + OUT_WAVE, l, wave, y, 1.f);
+        __syncthreads();
+        out_flush(smem, l, dk_row, 2 * wave, 2 * wave + 2);
+        out_flush(smem + OUT_WAVE, l, dv_row, 2 * wave, 2 * wave + 2);
+    } else {
+        unsigned char* lds = smem + wave * OUT_WAVE;
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+            out_put16(lds, l, dt, dka[0][dt], a.scale);
+            out_put16(lds, l, 2 + dt, dka[1][dt], -a.scale);
+        }
+        out_flush(lds, l, dk_row);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) out_put16(lds, l, dt, dva[dt], 1.f);
+        out_flush(lds, l, dv_row);
     }
-    out_flush(lds, l, [&](int r) { return k0 + r < a.Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; });
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) out_put16(lds, l, dt, dva[dt], 1.f);
-    out_flush(lds, l, [&](int r) { return k0 + r < a.Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; });
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1028,26 +1249,58 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
     return a;
 }
 
-unsigned blocks_of(int groups, int nx) { return (unsigned)(8 * ceil_div(groups, 8) * nx); }
-// Waves per block and split of the keys.  Few rows: one block a 32- or 64-row list.  Fewer blocks than the card holds (two of 128 rows a
-// compute unit, three of 32): the keys of each are cut into ranges of at least two tiles, as many as fill it; at most 64 ranges, and
-// 65536 partial rows.
 constexpr int PART = 2 * HV + 2;        // floats of workspace per row and range
-struct FwdPlan {
-    int nw, nx, nsplit;
+
+// Which block form, from the time model that the measurements below gave (us on 256 compute units; `steps` 32 x 32 tiles in a row):
+//   128 rows (keys) a block : steps * one;  beyond one block a compute unit two share it, 1.45 times as long, then as many as there are
+//   KEYS4 / ROWS4, 32 rows  : one block a compute unit, rounds of 256; ends + four * steps / 4 each, half of it on average if causal
+// measured, 128-row against four-way blocks: forward 1 x 1568 x 6 heads 53 / 47, 2 clips 54 / 73, 512 tokens 21 / 13, 5014 causal x 3 heads
+// 156 / 69, 32 x 160 17 / 38; dQ + dK / dV 1 x 1568 x 3 heads 130 / 63, 6 x 785 x 6 heads 91 / 142; dK / dV of 8 x 1111 causal, 4 heads a key
+// head 182 / 110.
+struct Model {
+    double one, four, ends;
 };
-FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv) {
-    FwdPlan p;
-    const long long R = (long long)(H / Hkv) * Nq, rows = (long long)B * H * Nq;
-    p.nw = R <= 32 ? 1 : R <= 64 ? 2 : 4;
-    p.nx = (int)((R + 32 * p.nw - 1) / (32 * p.nw));
-    const long long blocks = (long long)B * Hkv * p.nx, room = 256 * (p.nw == 4 ? 2 : 3), tiles = (Nk + 31) / 32;
-    long long n = room / blocks;
-    if (n > (tiles + 1) / 2) n = (tiles + 1) / 2;
-    if (n > 64) n = 64;
-    if (n > 65536 / rows) n = 65536 / rows;
-    p.nsplit = n < 2 ? 1 : (int)n;
+constexpr Model FWD = {0.96, 1.4, 4.0}, DQ = {0.9, 1.35, 2.0}, DKV = {1.15, 1.5, 2.5};
+double shared_time(const Model& m, long long blocks, long long steps) {
+    const double full = blocks / 300.0;
+    return m.one * steps * (blocks <= 256 ? 1.0 : full > 1.45 ? full : 1.45);
+}
+double four_time(const Model& m, long long blocks, long long steps, int causal) {
+    const long long rounds = (blocks + 255) / 256;
+    return rounds * (m.ends + m.four * ((steps + 3) / 4) * (causal && rounds > 1 ? 0.5 : 1.0));
+}
+
+// Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 5 us, and
+// a partial row is written and read at about 2000 rows a us.  At most 64 ranges and 65536 partial rows.  One token against 16 caches of
+// 8192, us by ranges: 1 103, 4 38, 8 32, 16 37; 11 rows x 1700 keys x 36 heads: 1 28, 6 18.
+struct FwdPlan {
+    bool keys4;
+    int nx, nsplit;
+};
+FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv, int causal) {
+    const long long R = (long long)(H / Hkv) * Nq, rows = (long long)B * H * Nq, groups = (long long)B * Hkv, tiles = (Nk + 31) / 32;
+    const long long n1 = (R + 127) / 128, n4 = (R + 31) / 32;
+    causal = causal == 1;                                 // towards the end: every row sees nearly all keys
+    FwdPlan p = {false, (int)n1, 1};
+    double best = shared_time(FWD, groups * n1, tiles);
+    for (int n = 1; n <= 64 && (n == 1 || (n <= tiles && n * rows <= 65536)); ++n) {
+        const double t = four_time(FWD, groups * n4 * n, (tiles + n - 1) / n, causal) + (n > 1 ? 5.0 + n * rows / 2000.0 : 0.0);
+        if (t < best) {
+            best = t;
+            p = {true, (int)n4, n};
+        }
+    }
     return p;
+}
+// place_block: over all XCDs?  With eight heads or more, of equal length, eighths of the list are even and K / V stay in one L2; 64 heads
+// of ragged lengths average out
+int spread_of(const DiffArgs& a) {
+    const long long groups = (long long)a.B * a.Hkv;
+    return (a.kv_len && groups < 64) || (a.causal && groups < 8);
+}
+unsigned grid_of(const DiffArgs& a, int nx, int spread) {
+    const long long n = (long long)a.B * a.Hkv * nx;
+    return (unsigned)(spread ? n : 8 * ((n + 7) / 8));
 }
 // blocks of one head's rows in the row pass: about 1024 in all, 64 rows each at least
 int row_blocks(int B, int Nq, int H) {
@@ -1069,7 +1322,7 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
     if (!o != !o2 || !o != !lse2) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: o, o2 and lse2 go together");
     if (ldo < H * HV || ldo % 8 || (((uintptr_t)out | (uintptr_t)o | (uintptr_t)o2) & 15))
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_fwd: bad ldo=%d (a multiple of 8), or an output that is not 16-byte aligned", ldo);
-    const FwdPlan pl = fwd_plan(B, Nq, Nk, H, Hkv);
+    const FwdPlan pl = fwd_plan(B, Nq, Nk, H, Hkv, causal);
     const long long rows = (long long)B * H * Nq;
     if (pl.nsplit > 1 && (!ws || ws_elems < rows * pl.nsplit * PART)) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: ws of %lld floats is too small", ws ? ws_elems : 0);
     if (pl.nsplit > 1 && ((uintptr_t)ws & 15)) MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_fwd: ws must be 16-byte aligned");
@@ -1087,19 +1340,19 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
         f.part = ws;
         f.part_lse = ws + rows * pl.nsplit * (2 * HV);
     }
-    const dim3 grid(blocks_of(B * Hkv, pl.nx * pl.nsplit));
+    const int spread = spread_of(a);
+    const dim3 grid(grid_of(a, pl.nx * pl.nsplit, spread));
     hipStream_t s = (hipStream_t)stream;
-#define MOFO_DIFF_FWD(NW)                                                                                                          \
-    do {                                                                                                                           \
-        if (o && pl.nsplit > 1) hipLaunchKernelGGL((diff_fwd_kernel<NW, true, true>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, pl.nsplit);  \
-        else if (o) hipLaunchKernelGGL((diff_fwd_kernel<NW, true, false>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, 1);               \
-        else if (pl.nsplit > 1) hipLaunchKernelGGL((diff_fwd_kernel<NW, false, true>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, pl.nsplit); \
-        else hipLaunchKernelGGL((diff_fwd_kernel<NW, false, false>), grid, dim3(NW * 64), 0, s, a, f, pl.nx, 1);                     \
-    } while (0)
-    if (pl.nw == 1) MOFO_DIFF_FWD(1);
-    else if (pl.nw == 2) MOFO_DIFF_FWD(2);
-    else MOFO_DIFF_FWD(4);
-#undef MOFO_DIFF_FWD
+    if (pl.nsplit > 1) {
+        if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, true>), grid, dim3(256), 0, s, a, f, pl.nx, pl.nsplit, spread);
+        else hipLaunchKernelGGL((diff_fwd_kernel<true, false, true>), grid, dim3(256), 0, s, a, f, pl.nx, pl.nsplit, spread);
+    } else if (pl.keys4) {
+        if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+        else hipLaunchKernelGGL((diff_fwd_kernel<true, false, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+    } else {
+        if (o) hipLaunchKernelGGL((diff_fwd_kernel<false, true, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+        else hipLaunchKernelGGL((diff_fwd_kernel<false, false, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+    }
     MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd");
     if (pl.nsplit > 1) {
         hipLaunchKernelGGL(diff_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, f, pl.nsplit);
@@ -1110,8 +1363,8 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
 
 extern "C" long long mofo_diff_attention_fwd_ws(int B, int Nq, int Nk, int H, int Hkv) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd_ws: bad dims");
-    const FwdPlan pl = fwd_plan(B, Nq, Nk, H, Hkv);
-    return pl.nsplit > 1 ? (long long)B * H * Nq * pl.nsplit * PART : 0;
+    const int n0 = fwd_plan(B, Nq, Nk, H, Hkv, 0).nsplit, n1 = fwd_plan(B, Nq, Nk, H, Hkv, 1).nsplit, n = n0 > n1 ? n0 : n1;
+    return n > 1 ? (long long)B * H * Nq * n * PART : 0;
 }
 
 extern "C" long long mofo_diff_attention_bwd_ws(int B, int Nq, int Nk, int H, int Hkv, int norm) {
@@ -1157,11 +1410,17 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
-    const int nx = ceil_div(a.R, 128), nk = ceil_div(Nk, 128);
-    hipLaunchKernelGGL(diff_dq_kernel, dim3(blocks_of(B * Hkv, nx)), dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx);
+    const long long groups = (long long)B * Hkv, kt = (Nk + 31) / 32, qt = (long long)a.G * ((Nq + 31) / 32);
+    const bool q4 = four_time(DQ, groups * ((a.R + 31) / 32), kt, causal == 1) < shared_time(DQ, groups * ((a.R + 127) / 128), kt);
+    const bool k4 = four_time(DKV, groups * kt, qt, causal) < shared_time(DKV, groups * ((Nk + 127) / 128), qt);
+    const int nx = ceil_div(a.R, q4 ? 32 : 128), nk = ceil_div(Nk, k4 ? 32 : 128);
+    const int spread = spread_of(a);
+    const dim3 gq(grid_of(a, nx, spread)), gk(grid_of(a, nk, spread));
+    if (q4) hipLaunchKernelGGL(diff_dq_kernel<true>, gq, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx, spread);
+    else hipLaunchKernelGGL(diff_dq_kernel<false>, gq, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx, spread);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dq)");
-    hipLaunchKernelGGL(diff_dkv_kernel, dim3(blocks_of(B * Hkv, nk)), dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv,
-                       (size_t)lddv, nk);
+    if (k4) hipLaunchKernelGGL(diff_dkv_kernel<true>, gk, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv, (size_t)lddv, nk, spread);
+    else hipLaunchKernelGGL(diff_dkv_kernel<false>, gk, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv, (size_t)lddv, nk, spread);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dkv)");
     hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + (dgamma ? 16 : 0)), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(params)");
