@@ -238,8 +238,8 @@ __device__ __forceinline__ void landed_barrier() {
 }
 
 // KEYS4 blocks (few rows, or few blocks): four waves share 32 rows and deal the key tiles -- or a wave's 32 keys the row tiles -- among
-// themselves.  Every wave has a ring of two tiles of its own and meets the others only at the end, where the four sums are added up
-// through LDS in a fixed order.
+// themselves.  Every wave has one tile of its own, refilled when its last read is done (two such blocks on a compute unit cover each
+// other's waits), and meets the others only at the end, where the four sums are added up through LDS in a fixed order.
 __device__ __forceinline__ void landed_own() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void acc_put(unsigned char* lds, int unit, int lane, const f32x16& x, float mul) {
 #pragma unroll
@@ -259,6 +259,9 @@ __device__ __forceinline__ f32x16 acc_sum(const unsigned char* lds, int stride, 
     }
     return x;
 }
+
+// a four-way wave's LDS reads are done: its one tile may be overwritten
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------------------ forward
 struct FwdOut {
@@ -285,10 +288,10 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // One block: four waves of 32 rows that share the key tiles of one (clip, key head), two tiles a barrier in a ring of four filled by LDS-DMA;
 // or KEYS4.  nsplit > 1: of a range of the keys, joined by diff_join_kernel.
 template <bool KEYS4, bool SAVE, bool SPLIT>
-__global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
-    constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128, XCH = 8 * STAGE;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[KEYS4 ? XCH + 4096 : 4 * STAGE];
-    __shared__ float gam[HV];
+__global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
+    constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128, XCH = 4 * STAGE;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[XCH + (KEYS4 ? 4096 : 0)];
+    __shared__ float gam[HV], lams[KEYS4 ? 32 : 1];         // KEYS4: the rows' lambda, out of the registers during the loop
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xs, b, kvh;
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a
     const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
     HalfTile ht = half_tile((KEYS4 || wave < 2 ? kp : vp) + (KEYS4 ? 0 : (wave & 1) * 64), KEYS4 || wave < 2 ? a.ldk : a.ldv, lane), hv;
     if constexpr (KEYS4) hv = half_tile(vp, a.ldv, lane);
-    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * 2 * STAGE : 0;
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * STAGE : 0;
     auto issue = [&](int t, unsigned buf) {
         const int row0 = (first + t * stride) * 32;
         const unsigned at = lds0 + ring + buf * STAGE;
@@ -344,6 +347,7 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a
             const float t = head_lambda(a, h, lane, e1, e2);
             lam = w.h == h ? t : lam;
         }
+        if (KEYS4 && tid < 32) lams[tid] = lam;
         if (a.gamma && tid < HV) gam[tid] = a.out_scale * param(a.gamma, a.param_bf16, tid);
     }
 
@@ -362,16 +366,15 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a
     for (int t = 0; t < nkt; ++t) {
         if constexpr (KEYS4) {
             landed_own();
-            if (t + 1 < nkt) issue(t + 1, (t + 1) & 1);
         } else if ((t & 1) == 0) {
             landed_barrier<0>();
             if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
             if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
         }
-        const unsigned buf = KEYS4 ? t & 1 : t & 3;
+        const unsigned buf = KEYS4 ? 0 : t & 3;
         const int k0 = (first + t * stride) * 32;
         const unsigned T = buf * STAGE;
-        if (k0 >= whi) continue;                          // no row of this wave sees the tile
+        if (k0 >= whi) continue;                          // no row of this wave sees the tile (KEYS4: one does)
         // fragment registers are refilled right behind the matrix instruction that read them
         bf16x8 fr[4];
         RowOff ro(fo, T);
@@ -422,6 +425,10 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a
         const float nmc[2] = {-mx[0] * a.c, -mx[1] * a.c};
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
+            if (KEYS4 && s2 == 1) {
+                reads_done();
+                if (t + 1 < nkt) issue(t + 1, 0);
+            }
             bf16x8 pf[2];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -484,18 +491,27 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_fwd_kernel(DiffArgs a
             inv[m] = some ? fast_exp2((mx[m] - top) * a.c) / st : 0.f;
             lse[m] = top * a.c + fast_log2(sx);
         }
+        // a map at a time (there is no room for both); wave w goes on with columns 32 w .. 32 w + 31
+        f32x16 sum[2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) {
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
-                if (!some) o[m][dt] = zero16();           // whatever a row that sees nothing holds
-                acc_put(smem + wave * 2 * STAGE, m * 4 + dt, lane, o[m][dt], inv[m]);
+                int on = some;                            // opaque: the selects of all eight tiles at once do not fit the registers
+                asm volatile("" : "+v"(on));
+                f32x16 x = o[m][dt];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = on ? x[r] : 0.f;           // whatever a row that sees nothing holds
+                acc_put(smem + wave * STAGE, dt, lane, x, inv[m]);
             }
+            __syncthreads();
+            sum[m] = acc_sum(smem, STAGE, wave, lane);
+            if (m == 0) __syncthreads();
+        }
         some = any;
-        __syncthreads();
-        // wave w goes on with columns 32 w .. 32 w + 31 of both maps
-        o[0][0] = acc_sum(smem, 2 * STAGE, wave, lane);
-        o[1][0] = acc_sum(smem, 2 * STAGE, 4 + wave, lane);
+        lam = lams[lane & 31];
+        o[0][0] = sum[0];
+        o[1][0] = sum[1];
         inv[0] = inv[1] = 1.f;
     } else {
 #pragma unroll
@@ -661,6 +677,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
 // stats[b, h, i] = (-lse_1 / c, -(lse_2 - log2|lam|) / c, -d1, d1 - d2), c = scale log2(e): what the score and G accumulators start from, so that
 // P1 = exp2(c acc), |lam| P2 = exp2(c acc) and G - d1, G - d2 come out of the matrix instructions.
 // 16 lanes a row, a block's rows all of one head; block partials of dgamma / dlam, summed in order by diff_param_kernel.
+// A copy's work: 32 x 1568 x 3 heads 31 us, 5.0 TB/s (one row at a time 35, four, with half the waves, 38).
+constexpr int ROWS_AT_ONCE = 2;
 __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t* __restrict__ o, const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dout,
                                                         size_t lddo, const float* __restrict__ lse2, bf16_t* __restrict__ d_o, f32x4* __restrict__ stats,
                                                         float* __restrict__ part, float* __restrict__ lams) {
@@ -677,59 +695,74 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
         dg[e] = 0.f;
     }
     const size_t total = (size_t)a.B * a.Nq, HW = (size_t)a.H * HV, plane = (size_t)a.B * a.H * a.Nq;
-    for (size_t base = (size_t)blockIdx.x * 16; base < total; base += (size_t)nb * 16) {
-        const size_t row = base + slot;
-        if (row >= total) continue;         // whole groups of 16 lanes: the shuffles below stay inside a group
-        const int b = (int)(row / a.Nq), i = (int)(row - (size_t)b * a.Nq);
-        const size_t st = ((size_t)b * a.H + h) * a.Nq + i;
-        const bool some = row_lim(a, clip_len(a, b), i) > 0;
-        const size_t off = row * HW + (size_t)h * HV + 8 * sub;
-        const u32x4 wo = *(const u32x4*)(o + off), w2 = *(const u32x4*)(o2 + off), wd = *(const u32x4*)(dout + row * lddo + (size_t)h * HV + 8 * sub);
-        float vo[8], v2[8], vd[8], gg[8];
-        float ss = 0.f, gx = 0.f;
+    for (size_t base = (size_t)blockIdx.x * (16 * ROWS_AT_ONCE); base < total; base += (size_t)nb * (16 * ROWS_AT_ONCE)) {
+        // both rows' loads first; a group behind the last row works on that row and stores nothing
+        u32x4 wo[ROWS_AT_ONCE], w2[ROWS_AT_ONCE], wd[ROWS_AT_ONCE];
+        float l1[ROWS_AT_ONCE], l2[ROWS_AT_ONCE];
+        size_t st[ROWS_AT_ONCE], off[ROWS_AT_ONCE];
+        bool some[ROWS_AT_ONCE];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            vo[e] = (e & 1) ? bf16hi_to_f32(wo[e >> 1]) : bf16lo_to_f32(wo[e >> 1]);
-            v2[e] = (e & 1) ? bf16hi_to_f32(w2[e >> 1]) : bf16lo_to_f32(w2[e >> 1]);
-            vd[e] = (e & 1) ? bf16hi_to_f32(wd[e >> 1]) : bf16lo_to_f32(wd[e >> 1]);
-            gg[e] = gam[e] * vd[e];
-            ss += vo[e] * vo[e];
-            gx += gg[e] * vo[e];
+        for (int j = 0; j < ROWS_AT_ONCE; ++j) {
+            const size_t want = base + 16 * j + slot, row = want < total ? want : total - 1;
+            const int b = (int)(row / a.Nq), i = (int)(row - (size_t)b * a.Nq);
+            st[j] = ((size_t)b * a.H + h) * a.Nq + i;
+            off[j] = row * HW + (size_t)h * HV + 8 * sub;
+            wo[j] = *(const u32x4*)(o + off[j]);
+            w2[j] = *(const u32x4*)(o2 + off[j]);
+            wd[j] = *(const u32x4*)(dout + row * lddo + (size_t)h * HV + 8 * sub);
+            l1[j] = lse2[st[j]];
+            l2[j] = lse2[plane + st[j]];
+            some[j] = row_lim(a, clip_len(a, b), i) > 0;
         }
-        u32x4 rd = wd;
-        if (a.gamma) {
 #pragma unroll
-            for (int x = 8; x > 0; x >>= 1) {
-                ss += __shfl_xor(ss, x, 64);
-                gx += __shfl_xor(gx, x, 64);
-            }
-            const float rn = 1.0f / sqrtf(ss * (1.f / HV) + a.eps);
-            const float k = gx * rn * rn * (1.f / HV);
+        for (int j = 0; j < ROWS_AT_ONCE; ++j) {
+            const bool mine = base + 16 * j + slot < total;
+            float vo[8], v2[8], vd[8], gg[8];
+            float ss = 0.f, gx = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                dg[e] += a.out_scale * vd[e] * vo[e] * rn;
-                gg[e] = some ? rn * (gg[e] - vo[e] * k) : 0.f;
+                vo[e] = (e & 1) ? bf16hi_to_f32(wo[j][e >> 1]) : bf16lo_to_f32(wo[j][e >> 1]);
+                v2[e] = (e & 1) ? bf16hi_to_f32(w2[j][e >> 1]) : bf16lo_to_f32(w2[j][e >> 1]);
+                vd[e] = (e & 1) ? bf16hi_to_f32(wd[j][e >> 1]) : bf16lo_to_f32(wd[j][e >> 1]);
+                gg[e] = gam[e] * vd[e];
+                ss += vo[e] * vo[e];
+                gx += gg[e] * vo[e];
             }
+            u32x4 rd = wd[j];
+            if (a.gamma) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) rd[e] = pack_bf16x2(gg[2 * e], gg[2 * e + 1]);
-            *(u32x4*)(d_o + off) = rd;
-        }
-        // d1, d2 from the rounded dO that the products read (their rows then sum to zero as the formula's do); dlam from the unrounded
-        float d1 = 0.f, d2 = 0.f, dx = 0.f;
+                for (int x = 8; x > 0; x >>= 1) {
+                    ss += __shfl_xor(ss, x, 64);
+                    gx += __shfl_xor(gx, x, 64);
+                }
+                const float rn = 1.0f / sqrtf(ss * (1.f / HV) + a.eps);
+                const float k = gx * rn * rn * (1.f / HV);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float q = (e & 1) ? bf16hi_to_f32(rd[e >> 1]) : bf16lo_to_f32(rd[e >> 1]);
-            d1 += q * (vo[e] + lam * v2[e]);
-            d2 += q * v2[e];
-            dx += gg[e] * v2[e];
-        }
-        if (some) dl -= dx;
+                for (int e = 0; e < 8; ++e) {
+                    if (mine) dg[e] += a.out_scale * vd[e] * vo[e] * rn;
+                    gg[e] = some[j] ? rn * (gg[e] - vo[e] * k) : 0.f;
+                }
 #pragma unroll
-        for (int x = 8; x > 0; x >>= 1) {
-            d1 += __shfl_xor(d1, x, 64);
-            d2 += __shfl_xor(d2, x, 64);
+                for (int e = 0; e < 4; ++e) rd[e] = pack_bf16x2(gg[2 * e], gg[2 * e + 1]);
+                if (mine) *(u32x4*)(d_o + off[j]) = rd;
+            }
+            // d1, d2 from the rounded dO that the products read (their rows then sum to zero as the formula's do); dlam from the unrounded
+            float d1 = 0.f, d2 = 0.f, dx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float q = (e & 1) ? bf16hi_to_f32(rd[e >> 1]) : bf16lo_to_f32(rd[e >> 1]);
+                d1 += q * (vo[e] + lam * v2[e]);
+                d2 += q * v2[e];
+                dx += gg[e] * v2[e];
+            }
+            if (mine && some[j]) dl -= dx;
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) {
+                d1 += __shfl_xor(d1, x, 64);
+                d2 += __shfl_xor(d2, x, 64);
+            }
+            if (sub == 0 && mine) stats[st[j]] = some[j] ? f32x4{-l1[j] * ic, (loglam - l2[j]) * ic, -d1, d1 - d2} : f32x4{-EMPTY_LSE * ic, -EMPTY_LSE * ic, 0.f, 0.f};
         }
-        if (sub == 0) stats[st] = some ? f32x4{-lse2[st] * ic, (loglam - lse2[plane + st]) * ic, -d1, d1 - d2} : f32x4{-EMPTY_LSE * ic, -EMPTY_LSE * ic, 0.f, 0.f};
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) red[slot][8 * sub + e] = dg[e];
@@ -788,10 +821,10 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
 // dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability)
 // Blocks and rings as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
 template <bool KEYS4>
-__global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+__global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
                                                                     const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx, int spread) {
     constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[(KEYS4 ? 8 : 4) * STAGE];
+    __shared__ __attribute__((aligned(128))) unsigned char smem[4 * STAGE + (KEYS4 ? OUT_WAVE : 0)];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
@@ -807,7 +840,7 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a,
     const bf16_t *kp = a.k + kr * a.ldk + (size_t)kvh * HV, *vp = a.v + kr * a.ldv + (size_t)kvh * HV;
     HalfTile ht = half_tile((KEYS4 || wave < 2 ? kp : vp) + (KEYS4 ? 0 : (wave & 1) * 64), KEYS4 || wave < 2 ? a.ldk : a.ldv, lane), hv;
     if constexpr (KEYS4) hv = half_tile(vp, a.ldv, lane);
-    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * 2 * STAGE : 0;
+    const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem), ring = KEYS4 ? wave * STAGE : 0;
     auto issue = [&](int t, unsigned buf) {
         const int row0 = (first + t * stride) * 32;
         const unsigned at = lds0 + ring + buf * STAGE;
@@ -844,14 +877,13 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a,
     for (int t = 0; t < nkt; ++t) {
         if constexpr (KEYS4) {
             landed_own();
-            if (t + 1 < nkt) issue(t + 1, (t + 1) & 1);
         } else if ((t & 1) == 0) {
             landed_barrier<0>();
             if (t + 2 < nkt) issue(t + 2, (t + 2) & 3);
             if (t + 3 < nkt) issue(t + 3, (t + 3) & 3);
         }
         const int k0 = (first + t * stride) * 32;
-        const unsigned T = (KEYS4 ? t & 1 : t & 3) * STAGE;
+        const unsigned T = (KEYS4 ? 0 : t & 3) * STAGE;
         if (k0 >= whi) continue;
         bf16x8 fr[4];
         RowOff ro(fo, T);
@@ -887,7 +919,11 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a,
                 if ((r & 3) + 8 * (r >> 2) >= lim) s[0][r] = s[1][r] = -__builtin_inff();
         }
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) {
+            if (KEYS4 && m == 1) {
+                reads_done();
+                if (t + 1 < nkt) issue(t + 1, 0);
+            }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 float p[8];
@@ -900,6 +936,7 @@ __global__ __launch_bounds__(256, KEYS4 ? 1 : 2) void diff_dq_kernel(DiffArgs a,
                     if (m == 0) fr[2 * s2 + dt] = co.get(TILE, s2, dt);
                 }
             }
+        }
     }
     const bool some = w.lim > 0;
     const float m1 = some ? a.scale : 0.f, m2 = lams[w.h] < 0.f ? m1 : -m1;
@@ -955,11 +992,11 @@ __device__ __forceinline__ bf16x8 selector(uint32_t w) {
 }
 
 template <bool ROWS4>
-__global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
+__global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
                                                           const float* __restrict__ lams, bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx,
                                                           int spread) {
-    constexpr int BUF = 4 * TILE + 512, VAT = (ROWS4 ? 8 : 2) * BUF;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + (ROWS4 ? 1 : 4) * 2 * TILE];
+    constexpr int BUF = 4 * TILE + 512, VAT = (ROWS4 ? 4 : 2) * BUF;
+    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + (ROWS4 ? 2 * TILE + 1024 : 8 * TILE)];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
@@ -967,7 +1004,7 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
     const int len = clip_len(a, b), off = past(a, len);
     const int kb0 = xb * (ROWS4 ? 32 : 128), k0 = kb0 + (ROWS4 ? 0 : wave * 32), key = k0 + (lane & 31);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
-    const unsigned ring = ROWS4 ? wave * 2 * BUF : 0, vt = VAT + (ROWS4 ? 0 : wave * 2 * TILE);
+    const unsigned ring = ROWS4 ? wave * BUF : 0, vt = VAT + (ROWS4 ? 0 : wave * 2 * TILE);
     const FragOff fo = frag_off(lds0, lane);
     {
         const bf16_t* vp = a.v + (size_t)b * a.Nk * a.ldv + (size_t)kvh * HV;
@@ -1052,16 +1089,25 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
         constexpr int PAR = decltype(buf_tag)::value;
         if constexpr (ROWS4) landed_own();
         else landed_barrier<0>();
-        if (t + 1 < steps) issue(ng, nqt_next, 1 - PAR);
+        if (!ROWS4 && t + 1 < steps) issue(ng, nqt_next, 1 - PAR);
         if (g != sgn_of) {                                                // a head begins
             sgn = lams[kvh * a.G + g] < 0.f ? -1.f : 1.f;
             sgn_of = g;
         }
         const unsigned T = ring + PAR * BUF;
         const int i0 = qt * 32, last = min(i0 + 31, a.Nq - 1);
+        const int gi = ng, qi = nqt_next;
         advance(g, qt, stride);
         advance(ng, nqt_next, stride);
-        if (min(len, last + off) > k0) {
+        auto refill = [&]() {
+            if (ROWS4) {
+                reads_done();
+                if (t + 1 < steps) issue(gi, qi, 0);
+            }
+        };
+        if (min(len, last + off) <= k0) {
+            refill();
+        } else {
             // four fragment registers: each is refilled right behind the matrix instruction that read it, a group ahead
             bf16x8 fr[4];
             RowOff ro(fo);
@@ -1070,19 +1116,16 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
             for (int ks = 0; ks < 4; ++ks) fr[ks] = ro.get(T, ks);
             const bf16x8 st = split3(hh ? rs[2] : rs[0], hh ? rs[3] : rs[1]);
             f32x16 s1 = mfma(st, selector(lower & 0x00003f80u), zero16()), s2 = mfma(st, selector(lower & 0x3f800000u), zero16());
-            
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 s1 = mfma(fr[ks], kf[0][ks], s1);
                 fr[ks] = ro.get(T + TILE, ks);
-                
             }
             ColOff co(fo);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 s2 = mfma(fr[ks], kf[1][ks], s2);
                 fr[ks] = co.get(T + (2 + (ks >> 1)) * TILE, 0, ks & 1);
-                
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s1[r] = fast_exp2(s1[r] * a.c);
@@ -1095,13 +1138,11 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
                 for (int r = 0; r < 16; ++r)
                     if ((r & 3) + 8 * (r >> 2) <= t) s1[r] = s2[r] = 0.f;
             }
-            
             {
                 float A[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) A[r] = fmaf(-sgn, s2[r], s1[r]);
                 const bf16x8 fa0 = pack_frag(A, 0), fa1 = pack_frag(A, 1);
-                
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt) {
                     dva[dt] = mfma(fr[dt], fa0, dva[dt]);
@@ -1129,7 +1170,6 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
                     fr[x] = co.get(T, ks & 1, 0);
                     fr[x + 1] = co.get(T, ks & 1, 1);
                 }
-                
             }
             {
                 float p1[16];
@@ -1137,7 +1177,6 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
                 for (int r = 0; r < 16; ++r) p1[r] = s1[r] * gr[r];
                 const bf16x8 f0 = pack_frag(p1, 0), f1 = pack_frag(p1, 1);
                 gr = mfma(st, selector(~lower & 0x3f800000u), gr);        // G - d1 -> G - d2
-                
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -1147,6 +1186,7 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
                         
                     }
             }
+            refill();
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float p2[8];
@@ -1161,7 +1201,7 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
     };
     for (int t = 0; t < steps; t += 2) {
         step(t, std::integral_constant<int, 0>{});
-        if (t + 1 < steps) step(t + 1, std::integral_constant<int, 1>{});
+        if (t + 1 < steps) step(t + 1, std::integral_constant<int, ROWS4 ? 0 : 1>{});
     }
     __syncthreads();                                      // the stages are free
     int l = lane;
@@ -1170,22 +1210,20 @@ __global__ __launch_bounds__(256, ROWS4 ? 1 : 2) void diff_dkv_kernel(DiffArgs a
     auto dk_row = [&](int r) { return k0 + r < a.Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; };
     auto dv_row = [&](int r) { return k0 + r < a.Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; };
     if constexpr (ROWS4) {
-        unsigned char* mine = smem + wave * 8 * 4096;
+        // dK, then dV: there is no room for both
+        unsigned char *mine = smem + wave * 4 * 4096, *out = smem + VAT;
+        static_assert(OUT_WAVE <= 2 * TILE + 1024 && 4 * 4 * 4096 <= VAT, "the sums and the rows that leave have their places");
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt) {
-            acc_put(mine, dt, l, dka[0][dt], a.scale);
-            acc_put(mine, 2 + dt, l, dka[1][dt], -a.scale);
+        for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) acc_put(mine, dt, l, pass ? dva[dt] : dka[dt >> 1][dt & 1], pass ? 1.f : dt < 2 ? a.scale : -a.scale);
+            __syncthreads();
+            out_put16(out, l, wave, acc_sum(smem, 4 * 4096, wave, l), 1.f);
+            __syncthreads();
+            if (pass) out_flush(out, l, dv_row, 2 * wave, 2 * wave + 2);
+            else out_flush(out, l, dk_row, 2 * wave, 2 * wave + 2);
+            __syncthreads();
         }
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) acc_put(mine, 4 + dt, l, dva[dt], 1.f);
-        __syncthreads();
-        const f32x16 x = acc_sum(smem, 8 * 4096, wave, l), y = acc_sum(smem, 8 * 4096, 4 + wave, l);
-        __syncthreads();
-        out_put16(smem, l, wave, x, 1.f);
-        out_put16(smem + OUT_WAVE, l, wave, y, 1.f);
-        __syncthreads();
-        out_flush(smem, l, dk_row, 2 * wave, 2 * wave + 2);
-        out_flush(smem + OUT_WAVE, l, dv_row, 2 * wave, 2 * wave + 2);
     } else {
         unsigned char* lds = smem + wave * OUT_WAVE;
 #pragma unroll
@@ -1251,28 +1289,30 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
 
 constexpr int PART = 2 * HV + 2;        // floats of workspace per row and range
 
-// Which block form, from the time model that the measurements below gave (us on 256 compute units; `steps` 32 x 32 tiles in a row):
-//   128 rows (keys) a block : steps * one;  beyond one block a compute unit two share it, 1.45 times as long, then as many as there are
-//   KEYS4 / ROWS4, 32 rows  : one block a compute unit, rounds of 256; ends + four * steps / 4 each, half of it on average if causal
-// measured, 128-row against four-way blocks: forward 1 x 1568 x 6 heads 53 / 47, 2 clips 54 / 73, 512 tokens 21 / 13, 5014 causal x 3 heads
-// 156 / 69, 32 x 160 17 / 38; dQ + dK / dV 1 x 1568 x 3 heads 130 / 63, 6 x 785 x 6 heads 91 / 142; dK / dV of 8 x 1111 causal, 4 heads a key
-// head 182 / 110.
-struct Model {
-    double one, four, ends;
-};
-constexpr Model FWD = {0.96, 1.4, 4.0}, DQ = {0.9, 1.35, 2.0}, DKV = {1.15, 1.5, 2.5};
-double shared_time(const Model& m, long long blocks, long long steps) {
-    const double full = blocks / 300.0;
-    return m.one * steps * (blocks <= 256 ? 1.0 : full > 1.45 ? full : 1.45);
+// Which block form, from a model of the time on 256 compute units that its measurements gave, us:
+//   128 rows (keys) a block, `steps` 32 x 32 tiles in a row    6.8 + 0.92 steps, two blocks on a compute unit 1.45 times that
+//   KEYS4 / ROWS4, 32 rows, a quarter of the steps             7.6 + 1.28 steps, two 9.9 + 1.7 steps
+// two blocks a compute unit at a time, rounds of 512 of them.  Causal blocks of a round differ in length and even out.
+// Measured, 128-row against four-way blocks, forward: 6 heads x 1568 52 / 31, 12 heads 53 / 52, 18 heads 54 / 62, 24 heads 74 / 80;
+// 32 x 6 heads x 160 17 / 24, 8 x 6 x 320 17 / 16, 4 heads x 16 clips of 50 8.9 / 11; causal 3 heads x 5014 155 / 63, 12 x 2500 82 / 65.
+// dQ follows the forward to a tenth.  dK / dV: 6 heads x 1568 60 / 31; causal 8 x 1111, 4 heads a key head 180 / 70.  A four-way ring of two
+// tiles, one block a compute unit, was 1.6 times slower beyond 256 blocks and at most 5 % faster below.
+double block_time(bool four, long long blocks, long long tiles, bool causal) {
+    const double steps = four ? (double)((tiles + 3) / 4) * (causal ? 0.75 : 1.0) : (double)tiles;
+    const double one = four ? 7.6 + 1.28 * steps : 6.8 + 0.92 * steps, two = four ? 9.9 + 1.7 * steps : (causal ? 1.2 : 1.45) * one;
+    if (blocks <= 256) return one;
+    if (causal) return two * (blocks <= 512 ? 1.0 : blocks / 512.0);
+    const long long rest = blocks % 512;
+    return (double)(blocks / 512) * two + (rest == 0 ? 0.0 : rest <= 256 ? one : two);
 }
-double four_time(const Model& m, long long blocks, long long steps, int causal) {
-    const long long rounds = (blocks + 255) / 256;
-    return rounds * (m.ends + m.four * ((steps + 3) / 4) * (causal && rounds > 1 ? 0.5 : 1.0));
+bool four_way(long long groups, long long rows, long long tiles, bool causal) {
+    return block_time(true, groups * ((rows + 31) / 32), tiles, causal) < block_time(false, groups * ((rows + 127) / 128), tiles, causal);
 }
 
-// Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 5 us, and
-// a partial row is written and read at about 2000 rows a us.  At most 64 ranges and 65536 partial rows.  One token against 16 caches of
-// 8192, us by ranges: 1 103, 4 38, 8 32, 16 37; 11 rows x 1700 keys x 36 heads: 1 28, 6 18.
+// Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 3 us and a
+// little per range, and a partial row is written and read at about 1500 rows a us.  At most 64 ranges and 65536 partial rows.  us by
+// ranges: one token against 16 caches of 8192 1 96, 4 36, 8 32, 16 32, 32 36; against one 1 91, 8 21, 32 16, 64 18; 11 rows x 1700 keys x
+// 36 heads 1 27, 6 17, 16 23; one head x 1568 1 24, 4 20, 8 22.
 struct FwdPlan {
     bool keys4;
     int nx, nsplit;
@@ -1280,11 +1320,11 @@ struct FwdPlan {
 FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv, int causal) {
     const long long R = (long long)(H / Hkv) * Nq, rows = (long long)B * H * Nq, groups = (long long)B * Hkv, tiles = (Nk + 31) / 32;
     const long long n1 = (R + 127) / 128, n4 = (R + 31) / 32;
-    causal = causal == 1;                                 // towards the end: every row sees nearly all keys
+    const bool half = causal == 1;                        // towards the end: every row sees nearly all keys
     FwdPlan p = {false, (int)n1, 1};
-    double best = shared_time(FWD, groups * n1, tiles);
+    double best = block_time(false, groups * n1, tiles, half);
     for (int n = 1; n <= 64 && (n == 1 || (n <= tiles && n * rows <= 65536)); ++n) {
-        const double t = four_time(FWD, groups * n4 * n, (tiles + n - 1) / n, causal) + (n > 1 ? 5.0 + n * rows / 2000.0 : 0.0);
+        const double t = block_time(true, groups * n4 * n, (tiles + n - 1) / n, half) + (n > 1 ? 3.0 + 0.05 * n + n * rows / 1500.0 : 0.0);
         if (t < best) {
             best = t;
             p = {true, (int)n4, n};
@@ -1411,8 +1451,7 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
     const long long groups = (long long)B * Hkv, kt = (Nk + 31) / 32, qt = (long long)a.G * ((Nq + 31) / 32);
-    const bool q4 = four_time(DQ, groups * ((a.R + 31) / 32), kt, causal == 1) < shared_time(DQ, groups * ((a.R + 127) / 128), kt);
-    const bool k4 = four_time(DKV, groups * kt, qt, causal) < shared_time(DKV, groups * ((Nk + 127) / 128), qt);
+    const bool q4 = four_way(groups, a.R, kt, causal == 1), k4 = four_way(groups, Nk, qt, causal != 0);
     const int nx = ceil_div(a.R, q4 ? 32 : 128), nk = ceil_div(Nk, k4 ? 32 : 128);
     const int spread = spread_of(a);
     const dim3 gq(grid_of(a, nx, spread)), gk(grid_of(a, nk, spread));

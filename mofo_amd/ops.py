@@ -21,7 +21,9 @@ _STREAM_OVERRIDE = None   # a torch.cuda.Stream while a launch sequence runs par
 
 def _stream():
     s = _STREAM_OVERRIDE
-    return (s if s is not None else torch.cuda.current_stream()).cuda_stream
+    if s is not None:
+        return s.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())   # current_stream().cuda_stream without the object: 0.3 instead of 2.8 us
 
 
 def launch_stream():
@@ -520,6 +522,9 @@ def _dev_chk(dev, dtype, dims, **tensors):
                 raise ValueError(f"{name} must be on the current device cuda:{dev}, it is on {t.device}")
 
 
+_INT4 = C.c_int * 4
+
+
 def _ld16(t):
     """row pitch of a 2-D tensor; a single row's own stride says nothing"""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -563,7 +568,7 @@ def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, int
         gh, gw = grid[1], grid[2]
     if M:
         _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), x.data_ptr(), 1 if dt is BF16 else 0, _ld16(x), out.data_ptr(), _ld16(out), M,
-             heads, head_dim, freqs.data_ptr(), axes, (C.c_int * 4)(*sections), _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
+             heads, head_dim, freqs.data_ptr(), axes, _INT4(*sections), _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
     return out
 
 
