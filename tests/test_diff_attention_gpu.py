@@ -325,6 +325,44 @@ def test_diff_attention_forward_and_gradients(dev, B, Nq, Nk, H, Hkv, causal, le
     _check(_call(*args), want)
 
 
+MANY = [  # enough (clip, key head) pairs for blocks of 128 rows (keys) in every kernel, or long rows for many four-way blocks; as DIFF
+    (24, 140, 140, 12, 12, 0, None, True, None, BF16),                        # eighths of 288 heads an XCD
+    (257, 130, 130, 1, 1, 0, None, False, 1, F32),                            # 257 of them: the last eighth is short
+    (67, 100, 100, 8, 4, 1, None, True, None, BF16),                          # two heads a key head, causal from the start
+    (10, 500, 500, 8, 4, 2, (0, 500, 1, 499, 33, 128, 257, 500, 64, 129), True, None, BF16),          # ragged: one list over all XCDs
+    (70, 50, 170, 4, 4, 2, tuple((b * 37) % 172 for b in range(70)), False, None, BF16),
+    (1, 2150, 2150, 8, 8, 1, None, True, 1, BF16)]                            # four-way, more blocks than the card holds at a time
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal,lens,norm,lam_heads,params", MANY)
+def test_diff_attention_many_blocks(dev, B, Nq, Nk, H, Hkv, causal, lens, norm, lam_heads, params):
+    test_diff_attention_forward_and_gradients(dev, B, Nq, Nk, H, Hkv, causal, lens, norm, lam_heads, params)
+
+
+def test_diff_attention_two_streams_at_once(dev):
+    """calls of two streams with workspaces of their own overlap and keep their bits"""
+    from mofo_amd import ops
+    states = []
+    for seed, (B, Nq, Nk, H, Hkv) in enumerate(((2, 300, 300, 6, 2), (3, 3, 2500, 4, 2))):
+        q, k, v, lam, gamma, dout = _case(dev, B, Nq, Nk, H, Hkv, True, seed=10 * seed)
+        want = _call(q, k, v, B, H, Hkv, 0.125, lam, 0.4, gamma, 0.6, None, 2, dout=dout)
+        new = lambda t: torch.full(t.shape, 9.0, dtype=BF16, device=dev)  # noqa: E731
+        need = max(ops.diff_attention_fwd_ws(B, Nq, Nk, H, Hkv), ops.diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, True))
+        states.append((torch.cuda.Stream(), (q, k, v, B, H, Hkv, 0.125, lam, 0.4), dict(gamma=gamma, eps=EPS, out_scale=0.6, causal=2), dout, want,
+                       (new(q), new(q), torch.empty(2, B, H, Nq, dtype=F32, device=dev)), [new(q), new(q), new(k), new(v)], torch.empty_like(lam),
+                       torch.empty_like(gamma), torch.empty(need, dtype=F32, device=dev)))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for stream, args, form, dout, _, saved, (out, dq, dk, dv), dlam, dgamma, ws in states:
+            with torch.cuda.stream(stream):
+                ops.diff_attention_fwd(*args, out, saved=saved, ws=ws, **form)
+                ops.diff_attention_bwd(*args, saved, dout, dq, dk, dv, dlam, ws, dgamma=dgamma, **form)
+    torch.cuda.synchronize()
+    for _, _, _, _, want, saved, (out, dq, dk, dv), dlam, dgamma, _ in states:
+        for n, t in dict(out=out, o=saved[0], o2=saved[1], lse2=saved[2], dq=dq, dk=dk, dv=dv, dlam=dlam, dgamma=dgamma).items():
+            assert torch.equal(t, want[n]), n
+
+
 TOKEN = [  # B, Nq, Nk, H, Hkv, kv_len, norm
     (1, 1, 257, 6, 6, None, True), (1, 1, 31, 1, 1, None, False), (2, 1, 1000, 8, 2, None, True), (3, 2, 777, 4, 1, (777, 2, 500), True),
     (4, 5, 90, 4, 4, (90, 5, 0, 33), False), (16, 1, 2048, 8, 2, tuple(1 + 136 * b for b in range(16)), True), (1, 1, 30000, 2, 1, (29999,), True),
