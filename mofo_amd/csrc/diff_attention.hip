@@ -124,8 +124,8 @@ struct ColOff {
 // heads first -- few heads, causal or of ragged lengths, where eighths of the list would be far from equal.  Causal blocks differ in
 // length along x (long ones at the end: `late`, or at the start): within an eighth long and short ones alternate along the list, and the
 // long ones start first.
-__device__ __forceinline__ bool place_block(const DiffArgs& a, int nx, int spread, bool late, int& x, int& b, int& kvh) {
-    const int groups = a.B * a.Hkv, n = groups * nx, id = blockIdx.x;
+__device__ __forceinline__ bool place_block(const DiffArgs& a, int id, int nx, int spread, bool late, int& x, int& b, int& kvh) {
+    const int groups = a.B * a.Hkv, n = groups * nx;
     int g, q;
     if (spread) {
         if (id >= n) return false;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xs, b, kvh;
-    if (!place_block(a, nx * nsplit, spread, true, xs, b, kvh)) return;
+    if (!place_block(a, blockIdx.x, nx * nsplit, spread, true, xs, b, kvh)) return;
     const int xb = xs / nsplit, sp = xs - xb * nsplit;
     const int len = clip_len(a, b);
     const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
@@ -676,7 +676,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
 //   d1 = dO . O1, d2 = dO . O2 (O1 = O + lam O2);  dlam -= d2
 // stats[b, h, i] = (-lse_1 / c, -(lse_2 - log2|lam|) / c, -d1, d1 - d2), c = scale log2(e): what the score and G accumulators start from, so that
 // P1 = exp2(c acc), |lam| P2 = exp2(c acc) and G - d1, G - d2 come out of the matrix instructions.
-// 16 lanes a row, a block's rows all of one head; block partials of dgamma / dlam, summed in order by diff_param_kernel.
+// 16 lanes a row, a block's rows all of one head; block partials of dgamma / dlam, summed in order by param_block.
 // A copy's work: 32 x 1568 x 3 heads 31 us, 5.0 TB/s (one row at a time 35, four, with half the waves, 38).
 constexpr int ROWS_AT_ONCE = 2;
 __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t* __restrict__ o, const bf16_t* __restrict__ o2, const bf16_t* __restrict__ dout,
@@ -777,18 +777,42 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
     }
 }
 
+// The sums of the parameters' partials, dK / dV and dQ need nothing of each other: one launch, in this order (the longest blocks early, the
+// last round of each filled by the next).
+struct GradArgs {
+    DiffArgs a;
+    const bf16_t* d_o;                                    // dO behind the norm
+    size_t lddo;
+    const f32x4* stats;
+    const float *lams, *part;
+    bf16_t *dq, *dk, *dv;
+    size_t lddq, lddk, lddv;
+    void *dlam, *dgamma;
+    int nb, grad_bf16, params, np, nxk, nk, nxq, spread;  // np, nk: the first parts' blocks, multiples of 8 (a block's XCD is its index mod 8)
+};
+// The kernel's arguments, read where they are used: those of all three parts, and the outputs' through the loops, do not fit the scalar registers
+__device__ __forceinline__ const GradArgs& grad_args() {
+    auto p = (const __attribute__((address_space(4))) GradArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const GradArgs*)p;
+}
+
 // block 0 .. lam_heads - 1: the four vectors' gradients of a head (or of all heads); 16 more blocks: 8 columns of dgamma each.  A block's
 // 32 groups of 8 threads walk the partial rows in strides of 32, in a fixed order.
-__global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float* __restrict__ part, int nb, void* dlam, void* dgamma, int grad_bf16) {
-    __shared__ double red[256];
+__device__ __forceinline__ void param_block(int id, double* red) {
+    const GradArgs& g = grad_args();
+    const DiffArgs a = g.a;
+    const float* part = g.part;
+    const int nb = g.nb, grad_bf16 = g.grad_bf16;
+    void *dlam = g.dlam, *dgamma = g.dgamma;
     const int tid = threadIdx.x;
     auto put = [&](void* p, size_t i, float v) {
         if (grad_bf16) ((bf16_t*)p)[i] = f32_to_bf16(v);
         else ((float*)p)[i] = v;
     };
-    const bool lam_block = (int)blockIdx.x < a.lam_heads;
-    const int first = lam_block && a.lam_heads > 1 ? blockIdx.x : 0, n = (lam_block && a.lam_heads > 1 ? 1 : a.H) * nb;
-    const int col = lam_block ? HV : 8 * ((int)blockIdx.x - a.lam_heads) + (tid & 7), start = lam_block ? tid : tid >> 3, step = lam_block ? 256 : 32;
+    const bool lam_block = id < a.lam_heads;
+    const int first = lam_block && a.lam_heads > 1 ? id : 0, n = (lam_block && a.lam_heads > 1 ? 1 : a.H) * nb;
+    const int col = lam_block ? HV : 8 * (id - a.lam_heads) + (tid & 7), start = lam_block ? tid : tid >> 3, step = lam_block ? 256 : 32;
     const float* p = part + (size_t)first * nb * (HV + 1) + col;
     double s = 0.0;
     int k = start;
@@ -809,9 +833,9 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
     if (lam_block) {
         const float dl = (float)red[0];
         float e1, e2;
-        head_lambda(a, blockIdx.x, tid & 63, e1, e2);
+        head_lambda(a, id, tid & 63, e1, e2);
         const int v = tid >> 6;                                    // wave v: vector v; its partner is v ^ 1
-        const size_t st = (size_t)a.lam_heads * 64, at = (size_t)blockIdx.x * 64 + (tid & 63);
+        const size_t st = (size_t)a.lam_heads * 64, at = (size_t)id * 64 + (tid & 63);
         put(dlam, v * st + at, dl * (v < 2 ? e1 : -e2) * param(a.lam, a.param_bf16, (v ^ 1) * st + at));
     } else if (tid < 8) {
         put(dgamma, col, (float)red[tid]);
@@ -820,15 +844,20 @@ __global__ __launch_bounds__(256) void diff_param_kernel(DiffArgs a, const float
 
 // dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability)
 // Blocks and rings as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
+constexpr int dq_lds(bool keys4) { return 16 * TILE + (keys4 ? OUT_WAVE : 0); }
 template <bool KEYS4>
-__global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                                    const float* __restrict__ lams, bf16_t* __restrict__ dq, size_t lddq, int nx, int spread) {
+__device__ __forceinline__ void dq_block(int id, unsigned char* smem) {
+    const GradArgs& in = grad_args();
+    const DiffArgs a = in.a;
+    const bf16_t* __restrict__ d_o = in.d_o;
+    const size_t lddo = in.lddo;
+    const f32x4* __restrict__ stats = in.stats;
+    const float* __restrict__ lams = in.lams;
     constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[4 * STAGE + (KEYS4 ? OUT_WAVE : 0)];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
-    if (!place_block(a, nx, spread, true, xb, b, kvh)) return;
+    if (!place_block(a, id, in.nxq, in.spread, true, xb, b, kvh)) return;
     const int len = clip_len(a, b);
     const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
@@ -945,6 +974,9 @@ __global__ __launch_bounds__(256, 2) void diff_dq_kernel(DiffArgs a, const bf16_
         for (int m = 0; m < 2; ++m) dqa[m][0] = dqa[m][1] = zero16();
     }
     __syncthreads();                                      // the ring is free
+    const GradArgs& fin = grad_args();
+    bf16_t* dq = fin.dq;
+    const size_t lddq = fin.lddq;
     if constexpr (KEYS4) {
         unsigned char* mine = smem + wave * STAGE;
 #pragma unroll
@@ -991,16 +1023,21 @@ __device__ __forceinline__ bf16x8 selector(uint32_t w) {
     return __builtin_bit_cast(bf16x8, u32x4{w, w, w, w});
 }
 
+constexpr int DKV_BUF = 4 * TILE + 512;
+constexpr int dkv_lds(bool rows4) { return rows4 ? 4 * DKV_BUF + 2 * TILE + 1024 : 2 * DKV_BUF + 8 * TILE; }
 template <bool ROWS4>
-__global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16_t* __restrict__ d_o, size_t lddo, const f32x4* __restrict__ stats,
-                                                          const float* __restrict__ lams, bf16_t* __restrict__ dk, size_t lddk, bf16_t* __restrict__ dv, size_t lddv, int nx,
-                                                          int spread) {
-    constexpr int BUF = 4 * TILE + 512, VAT = (ROWS4 ? 4 : 2) * BUF;
-    __shared__ __attribute__((aligned(128))) unsigned char smem[VAT + (ROWS4 ? 2 * TILE + 1024 : 8 * TILE)];
+__device__ __forceinline__ void dkv_block(int id, unsigned char* smem) {
+    const GradArgs& in = grad_args();
+    const DiffArgs a = in.a;
+    const bf16_t* __restrict__ d_o = in.d_o;
+    const size_t lddo = in.lddo;
+    const f32x4* __restrict__ stats = in.stats;
+    const float* __restrict__ lams = in.lams;
+    constexpr int BUF = DKV_BUF, VAT = (ROWS4 ? 4 : 2) * BUF;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int xb, b, kvh;
-    if (!place_block(a, nx, spread, false, xb, b, kvh)) return;
+    if (!place_block(a, id, in.nxk, in.spread, false, xb, b, kvh)) return;
     const int len = clip_len(a, b), off = past(a, len);
     const int kb0 = xb * (ROWS4 ? 32 : 128), k0 = kb0 + (ROWS4 ? 0 : wave * 32), key = k0 + (lane & 31);
     const unsigned lds0 = (unsigned)(size_t)LDS_PTR(smem);
@@ -1206,9 +1243,13 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
     __syncthreads();                                      // the stages are free
     int l = lane;
     asm volatile("" : "+v"(l));                           // nothing of this is kept through the loop
-    const size_t row0 = (size_t)b * a.Nk;
-    auto dk_row = [&](int r) { return k0 + r < a.Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; };
-    auto dv_row = [&](int r) { return k0 + r < a.Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; };
+    const GradArgs& fin = grad_args();
+    bf16_t *dk = fin.dk, *dv = fin.dv;
+    const size_t lddk = fin.lddk, lddv = fin.lddv, row0 = (size_t)b * fin.a.Nk;
+    const int Nk = fin.a.Nk;
+    const float scale = fin.a.scale;
+    auto dk_row = [&](int r) { return k0 + r < Nk ? dk + (row0 + k0 + r) * lddk + (size_t)kvh * HV : (bf16_t*)nullptr; };
+    auto dv_row = [&](int r) { return k0 + r < Nk ? dv + (row0 + k0 + r) * lddv + (size_t)kvh * HV : (bf16_t*)nullptr; };
     if constexpr (ROWS4) {
         // dK, then dV: there is no room for both
         unsigned char *mine = smem + wave * 4 * 4096, *out = smem + VAT;
@@ -1216,7 +1257,7 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) acc_put(mine, dt, l, pass ? dva[dt] : dka[dt >> 1][dt & 1], pass ? 1.f : dt < 2 ? a.scale : -a.scale);
+            for (int dt = 0; dt < 4; ++dt) acc_put(mine, dt, l, pass ? dva[dt] : dka[dt >> 1][dt & 1], pass ? 1.f : dt < 2 ? scale : -scale);
             __syncthreads();
             out_put16(out, l, wave, acc_sum(smem, 4 * 4096, wave, l), 1.f);
             __syncthreads();
@@ -1228,13 +1269,28 @@ __global__ __launch_bounds__(256, 2) void diff_dkv_kernel(DiffArgs a, const bf16
         unsigned char* lds = smem + wave * OUT_WAVE;
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt) {
-            out_put16(lds, l, dt, dka[0][dt], a.scale);
-            out_put16(lds, l, 2 + dt, dka[1][dt], -a.scale);
+            out_put16(lds, l, dt, dka[0][dt], scale);
+            out_put16(lds, l, 2 + dt, dka[1][dt], -scale);
         }
         out_flush(lds, l, dk_row);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) out_put16(lds, l, dt, dva[dt], 1.f);
         out_flush(lds, l, dv_row);
+    }
+}
+
+template <bool KEYS4, bool ROWS4>
+__global__ __launch_bounds__(256, 2) void diff_grad_kernel(GradArgs) {
+    constexpr int LDS_Q = dq_lds(KEYS4), LDS_K = dkv_lds(ROWS4);
+    __shared__ __attribute__((aligned(128))) unsigned char smem[LDS_Q > LDS_K ? LDS_Q : LDS_K];
+    const GradArgs& g = grad_args();
+    const int id = blockIdx.x, np = g.np, nk = g.nk;
+    if (id < np) {
+        if (id < g.params) param_block(id, (double*)smem);
+    } else if (id < np + nk) {
+        dkv_block<ROWS4>(id - np, smem);
+    } else {
+        dq_block<KEYS4>(id - np - nk, smem);
     }
 }
 
@@ -1338,9 +1394,9 @@ int spread_of(const DiffArgs& a) {
     const long long groups = (long long)a.B * a.Hkv;
     return (a.kv_len && groups < 64) || (a.causal && groups < 8);
 }
-unsigned grid_of(const DiffArgs& a, int nx, int spread) {
+unsigned grid_of(const DiffArgs& a, int nx) {
     const long long n = (long long)a.B * a.Hkv * nx;
-    return (unsigned)(spread ? n : 8 * ((n + 7) / 8));
+    return (unsigned)(8 * ((n + 7) / 8));
 }
 // blocks of one head's rows in the row pass: about 1024 in all, 64 rows each at least
 int row_blocks(int B, int Nq, int H) {
@@ -1381,7 +1437,7 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
         f.part_lse = ws + rows * pl.nsplit * (2 * HV);
     }
     const int spread = spread_of(a);
-    const dim3 grid(grid_of(a, pl.nx * pl.nsplit, spread));
+    const dim3 grid(grid_of(a, pl.nx * pl.nsplit));
     hipStream_t s = (hipStream_t)stream;
     if (pl.nsplit > 1) {
         if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, true>), grid, dim3(256), 0, s, a, f, pl.nx, pl.nsplit, spread);
@@ -1452,16 +1508,18 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
     const long long groups = (long long)B * Hkv, kt = (Nk + 31) / 32, qt = (long long)a.G * ((Nq + 31) / 32);
     const bool q4 = four_way(groups, a.R, kt, causal == 1), k4 = four_way(groups, Nk, qt, causal != 0);
-    const int nx = ceil_div(a.R, q4 ? 32 : 128), nk = ceil_div(Nk, k4 ? 32 : 128);
-    const int spread = spread_of(a);
-    const dim3 gq(grid_of(a, nx, spread)), gk(grid_of(a, nk, spread));
-    if (q4) hipLaunchKernelGGL(diff_dq_kernel<true>, gq, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx, spread);
-    else hipLaunchKernelGGL(diff_dq_kernel<false>, gq, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dq, (size_t)lddq, nx, spread);
-    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dq)");
-    if (k4) hipLaunchKernelGGL(diff_dkv_kernel<true>, gk, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv, (size_t)lddv, nk, spread);
-    else hipLaunchKernelGGL(diff_dkv_kernel<false>, gk, dim3(256), 0, s, a, dy, lddy, stats, lams, (bf16_t*)dk, (size_t)lddk, (bf16_t*)dv, (size_t)lddv, nk, spread);
-    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(dkv)");
-    hipLaunchKernelGGL(diff_param_kernel, dim3(lam_heads + (dgamma ? 16 : 0)), dim3(256), 0, s, a, (const float*)part, nb, dlam, dgamma, grad_is_bf16);
-    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(params)");
+    GradArgs g = {a, dy, lddy, stats, lams, part, (bf16_t*)dq, (bf16_t*)dk, (bf16_t*)dv, (size_t)lddq, (size_t)lddk, (size_t)lddv, dlam, dgamma, nb, grad_is_bf16};
+    g.params = lam_heads + (dgamma ? 16 : 0);
+    g.np = (g.params + 7) / 8 * 8;
+    g.nxk = ceil_div(Nk, k4 ? 32 : 128);
+    g.nk = (int)grid_of(a, g.nxk);
+    g.nxq = ceil_div(a.R, q4 ? 32 : 128);
+    g.spread = spread_of(a);
+    const dim3 grid(g.np + g.nk + grid_of(a, g.nxq));
+    if (q4 && k4) hipLaunchKernelGGL((diff_grad_kernel<true, true>), grid, dim3(256), 0, s, g);
+    else if (q4) hipLaunchKernelGGL((diff_grad_kernel<true, false>), grid, dim3(256), 0, s, g);
+    else if (k4) hipLaunchKernelGGL((diff_grad_kernel<false, true>), grid, dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((diff_grad_kernel<false, false>), grid, dim3(256), 0, s, g);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(gradients)");
     return MOFO_OK;
 }
