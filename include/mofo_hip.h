@@ -206,6 +206,7 @@ int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, int ldo, in
  * Key j of clip b is visible to query i iff j < kv_len[b] (i32 [B]; NULL: Nk; values are cut to 0 .. Nk) and, causal = 1: j <= i;
  * causal = 2: j <= i + kv_len[b] - Nq (new tokens at the end of a cache).  A row that sees nothing gives zeros, and takes none of
  * the gradients.  Rows of k, v at and behind kv_len[b] may hold anything; rows in front of it are expected to be finite.
+ * scale: 2^-24 .. 2^24; eps (with gamma): at least 2^-100.
  * For the gradient keep o, o2 (bf16 [B * Nq, H * 128], contiguous) and lse2 (f32 [2, B, H, Nq], log2-sum-exp2); NULL all three otherwise.
  * ws: mofo_diff_attention_fwd_ws floats of scratch (0: NULL is fine), contents of no interest; two calls that may run at once (two
  * streams, two captured graphs) need one each. ---- */

@@ -1296,12 +1296,14 @@ __global__ __launch_bounds__(256, 2) void diff_grad_kernel(GradArgs) {
 
 // ------------------------------------------------------------------------------------------------ host
 int check(const char* who, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
-          const void* lam, int lam_heads, int causal) {
+          const void* lam, int lam_heads, int causal, bool norm, float eps) {
     if (!q || !k || !v || !lam) MOFO_FAIL(MOFO_EINVAL, "%s: null pointer", who);
     if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv)
         MOFO_FAIL(MOFO_EINVAL, "%s: bad dims B=%d Nq=%d Nk=%d H=%d Hkv=%d (H a multiple of Hkv)", who, B, Nq, Nk, H, Hkv);
     if (H > 4096) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: H=%d (at most 4096)", who, H);
-    if (!(scale > 0.f) || !(scale < 3.0e38f)) MOFO_FAIL(MOFO_EINVAL, "%s: scale must be positive and finite", who);
+    // beyond them EMPTY_LSE over the exponent's factor, or a score times it, leaves f32
+    if (!(scale >= 0x1p-24f && scale <= 0x1p24f)) MOFO_FAIL(MOFO_EINVAL, "%s: scale must lie in 2^-24 .. 2^24", who);
+    if (norm && !(eps >= 0x1p-100f && eps < 3.0e38f)) MOFO_FAIL(MOFO_EINVAL, "%s: eps must be at least 2^-100 (a row of zeros has no root mean square)", who);
     if (lam_heads != 1 && lam_heads != H) MOFO_FAIL(MOFO_EINVAL, "%s: lam of %d heads, must be 1 or H=%d", who, lam_heads, H);
     if (causal < 0 || causal > 2) MOFO_FAIL(MOFO_EINVAL, "%s: causal=%d must be 0, 1 or 2", who, causal);
     if (ldq < H * HV || ldk < Hkv * HV || ldv < Hkv * HV || (ldq | ldk | ldv) % 8)
@@ -1412,7 +1414,7 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
                                        float scale, const void* lam, int lam_heads, float lam_init, const void* gamma, int param_is_bf16, float eps,
                                        float out_scale, const int* kv_len, int causal, void* out, int ldo, void* o, void* o2, float* lse2,
                                        float* ws, long long ws_elems, void* stream) {
-    int rc = check("mofo_diff_attention_fwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal);
+    int rc = check("mofo_diff_attention_fwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal, gamma != nullptr, eps);
     if (rc) return rc;
     if (!out) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: null output");
     if (!o != !o2 || !o != !lse2) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_fwd: o, o2 and lse2 go together");
@@ -1474,12 +1476,13 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
                                        float out_scale, const int* kv_len, int causal, const void* o, const void* o2, const float* lse2, const void* dout,
                                        int lddo, void* dq, int lddq, void* dk, int lddk, void* dv, int lddv, void* dlam, void* dgamma, int grad_is_bf16,
                                        float* ws, long long ws_elems, void* stream) {
-    int rc = check("mofo_diff_attention_bwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal);
+    int rc = check("mofo_diff_attention_bwd", q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, causal, gamma != nullptr, eps);
     if (rc) return rc;
     if (!o || !o2 || !lse2 || !dout || !dq || !dk || !dv || !dlam || !ws) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: null pointer");
     if (!gamma != !dgamma) MOFO_FAIL(MOFO_EINVAL, "mofo_diff_attention_bwd: gamma and dgamma go together");
     if (lddo < H * HV || lddq < H * HV || lddk < Hkv * HV || lddv < Hkv * HV || (lddo | lddq | lddk | lddv) % 8)
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: bad leading dims of the gradients");
+    if (lddo > (1 << 24)) MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: row pitch above 2^24");
     if (((uintptr_t)o | (uintptr_t)o2 | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)ws) & 15)
         MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_diff_attention_bwd: tensors must be 16-byte aligned");
     if (ws_elems < mofo_diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, gamma != nullptr))

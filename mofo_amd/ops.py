@@ -651,7 +651,8 @@ def diff_attention_fwd(q, k, v, B, H, Hkv, scale, lam, lam_init, out, gamma=None
     ``q`` bf16 [B * Nq, H * 128] (two 64-wide queries a head), ``k``, ``v`` bf16 [B * Nk, Hkv * 128]: column ranges of one packed projection,
     or a cache of Nk rows a clip.  ``lam`` [4, 1 or H, 64] (f32 or bf16; ``gamma`` alike): lambda = exp(lam0 . lam1) - exp(lam2 . lam3) + lam_init.
     ``kv_len`` i32 [B]: keys each clip holds; ``causal`` 1: key <= query, 2: the queries are the last Nq of the clip's keys.  A row that sees
-    no key gives zeros.  ``saved`` = (o, o2, lse2): kept for ``diff_attention_bwd``.  ``ws``: f32, diff_attention_fwd_ws elements."""
+    no key gives zeros.  ``scale`` 2^-24 .. 2^24, ``eps`` at least 2^-100.  ``saved`` = (o, o2, lse2): kept for ``diff_attention_bwd``.
+    ``ws``: f32, diff_attention_fwd_ws elements."""
     dev, Nq, Nk = _diff_chk("diff_attention_fwd", q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
     _dev_chk(dev, BF16, 2, out=out)
     if out is None or out.shape != q.shape:

@@ -49,6 +49,7 @@ def _fwd(**kw):
     dict(ldk=1 << 25), dict(q=P + 8), dict(k=P + 2), dict(ldo=511), dict(out=P + 4), dict(o=6 * P), dict(o=6 * P, o2=7 * P), dict(lse2=8 * P),
     dict(o=6 * P + 8, o2=7 * P, lse2=8 * P), dict(out=P), dict(out=2 * P), dict(out=P + 1024, ldq=1024, ldo=1032), dict(o=6 * P, o2=6 * P + 64, lse2=8 * P),
     dict(o=6 * P, o2=7 * P, lse2=4 * P), dict(gamma=4 * P + 16), dict(kv_len=4 * P), dict(Nq=1, Nk=4096, ldk=256, ws=None), dict(Nq=1, Nk=4096, ws=9 * P, n=100),
+    dict(scale=2.0 ** -25), dict(scale=2.0 ** 25), dict(gamma=20 * P, eps=0.0), dict(gamma=20 * P, eps=-1e-5), dict(gamma=20 * P, eps=math.nan),
     dict(H=8192, ldq=1 << 20, ldo=1 << 20, lam_heads=1), dict(B=1 << 20, Nk=1 << 20), dict(Nq=1 << 30)])
 def test_diff_attention_entry_refuses(bad):
     assert _fwd(**bad) < 0 and "mofo_diff_attention_fwd" in _error()
@@ -64,7 +65,8 @@ def _bwd(**kw):
 
 @pytest.mark.parametrize("bad", [
     dict(o=None), dict(o2=None), dict(lse2=None), dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(dlam=None), dict(ws=None), dict(n=10),
-    dict(gamma=20 * P), dict(dgamma=20 * P), dict(dq=P), dict(dk=3 * P), dict(dv=10 * P + 128), dict(dlam=4 * P), dict(ws=8 * P), dict(dq=5 * P), dict(lddo=504), dict(lddq=256), dict(lddk=130), dict(lddv=128), dict(dout=8 * P + 8), dict(ws=13 * P + 4), dict(H=5), dict(q=None)])
+    dict(gamma=20 * P), dict(dgamma=20 * P), dict(dq=P), dict(dk=3 * P), dict(dv=10 * P + 128), dict(dlam=4 * P), dict(ws=8 * P), dict(dq=5 * P), dict(lddo=504), dict(lddq=256), dict(lddk=130), dict(lddv=128), dict(dout=8 * P + 8), dict(ws=13 * P + 4), dict(H=5), dict(q=None),
+    dict(lddo=1 << 25), dict(scale=2.0 ** -25), dict(gamma=30 * P, dgamma=31 * P, eps=0.0)])
 def test_diff_attention_gradient_entry_refuses(bad):
     assert _bwd(**bad) < 0 and "mofo_diff_attention_bwd" in _error()
 

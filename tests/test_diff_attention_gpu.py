@@ -433,6 +433,21 @@ def test_diff_attention_signs_of_lambda(dev, lam_init):
     _check(_call(*args, dout=dout, grads=F32), _reference(*args, dout=dout, grad_u=0.0))
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -24, 2.0 ** 24])
+def test_diff_attention_ends_of_the_scale(dev, scale):
+    """the smallest and the largest scale taken: uniform maps, and one key a row; rows that see nothing, and a head whose lambda is exactly zero"""
+    B, N, H = 2, 70, 2
+    q, k, v, lam, gamma, dout = _case(dev, B, N, N, H, H, True, params=F32)
+    lam[:, 0] = 0.0
+    args = (q, k, v, B, H, H, scale, lam, 0.0, gamma, 0.6, torch.tensor([70, 30], dtype=I32, device=dev), 2)
+    got = _call(*args, dout=dout, grads=F32)
+    if scale < 1:
+        _check(got, _reference(*args, dout=dout, grad_u=0.0))
+    for n, t in got.items():
+        assert bool(torch.isfinite(t.float()).all()), n
+    assert not got["out"][N:N + 40].any() and not got["dq"][N:N + 40].any() and not got["dk"][N + 30:].any() and not got["dv"][N + 30:].any()
+
+
 def test_diff_attention_gradients_against_differences(dev):
     """the kernels' gradients along a direction against central differences of the definition in 64 bits"""
     B, N, H, Hkv = 2, 37, 4, 2
