@@ -287,6 +287,12 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 
 // One block: four waves of 32 rows that share the key tiles of one (clip, key head), two tiles a barrier in a ring of four filled by LDS-DMA;
 // or KEYS4.  nsplit > 1: of a range of the keys, joined by diff_join_kernel.
+// 24 matrix instructions (768 cycles of the matrix unit) and about 150 others, 32 of them exponentials at twice the time (740 cycles), stand
+// against 2100 cycles a tile and wave that a full card takes: matrix unit 36 % and vector unit 40 % busy, LDS 17 %, two waves a SIMD (the
+// registers allow no third) whose phases meet too often.  16 clips x 6 heads x 1568 tokens 208 us, 580 TFLOP/s; one clip of 12544 890 us,
+// 543 TFLOP/s; one clip of 1568 31 us.  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
+// without gain: the two maps' first products in turn, the next tile's first fragments ahead of the barrier, fences that
+// interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the register file.
 template <bool KEYS4, bool SAVE, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
     constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128, XCH = 4 * STAGE;
@@ -612,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 }
 
 // joins the ranges of a row: one wave a row, lanes 0..31 the first map's 128 columns, lanes 32..63 the second's; the ranges' weights are
-// exp2(lse_range - lse), lane s holding range s
+// exp2(lse_range - lse), lane s holding range s.  Eight loads in flight a lane: one token against 16 caches of 8192, 8 ranges, 3 us of 32.
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, int nsplit) {
     const int lane = threadIdx.x & 63, m = lane >> 5, d = (lane & 31) * 4;
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (size_t)a.B * a.H * a.Nq;
@@ -778,7 +784,8 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
 }
 
 // The sums of the parameters' partials, dK / dV and dQ need nothing of each other: one launch, in this order (the longest blocks early, the
-// last round of each filled by the next).
+// last round of each filled by the next).  32 x 160 x 6 heads 31 us (three launches 16 + 19 + 5), 8 ragged clips of 1111 92 (44 + 70 + 5),
+// 32 x 1568 x 3 heads 468 (205 + 270 + 7).
 struct GradArgs {
     DiffArgs a;
     const bf16_t* d_o;                                    // dO behind the norm
@@ -843,7 +850,8 @@ __device__ __forceinline__ void param_block(int id, double* red) {
 }
 
 // dQ: dS_m = P_m (G - d_m), G = dO V^T; dQ_1 = scale dS_1 K_1, dQ_2 = -lam scale dS_2 K_2 (|lam| sits in the probability)
-// Blocks and rings as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.
+// Blocks and rings as in the forward pass; 24 matrix instructions and 24 KiB of LDS reads a tile and wave.  Alone 32 x 1568 x 3 heads 205 us,
+// 590 TFLOP/s.
 constexpr int dq_lds(bool keys4) { return 16 * TILE + (keys4 ? OUT_WAVE : 0); }
 template <bool KEYS4>
 __device__ __forceinline__ void dq_block(int id, unsigned char* smem) {
@@ -1005,7 +1013,7 @@ __device__ __forceinline__ void dq_block(int id, unsigned char* smem) {
 // dV product comes before G = dO V^T, so that A is gone when G needs its place.  Two LDS stages of Q, dO and the rows' statistics.
 // A row's statistics are wanted by every lane of an accumulator row: each lane splits its own row's numbers into three bf16 terms (exact to
 // f32) and one more matrix instruction, against a selector of ones, spreads a number over the accumulator.  Reading them from LDS per
-// accumulator row cost as much LDS time as two operands.
+// accumulator row cost as much LDS time as two operands.  Alone 32 x 1568 x 3 heads 270 us: matrix unit 45 % and vector unit 44 % busy.
 __device__ const f32x4 g_pad_stat = {-1.0e36f, -1.0e36f, 0.f, 0.f};     // a row behind the last: exp2(c acc) = 0
 __device__ __forceinline__ bf16x8 split3(float x, float y) {
     u32x4 f = {0, 0, 0, 0};
@@ -1390,11 +1398,12 @@ FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv, int causal) {
     }
     return p;
 }
-// place_block: over all XCDs?  With eight heads or more, of equal length, eighths of the list are even and K / V stay in one L2; 64 heads
-// of ragged lengths average out
+// place_block: over all XCDs when lengths differ, or with few causal heads; eighths of the list otherwise, where K / V stay in one L2.  us,
+// eighths against spread, forward / gradient: 16 x 6 heads x 1568 241 / 501 against 248 / 506; one clip of 12544 925 / 2063, 940 / 2158;
+// causal 6 heads x 5014 111 / 214, 96 / 214, 8 heads 120 / 257, 122 / 259, 12 heads 169 / 369, 170 / 336; ragged causal 1111, 4 heads a key
+// head, 8 clips 60 / 136, 57 / 114, 32 clips 197 / 383, 178 / 364
 int spread_of(const DiffArgs& a) {
-    const long long groups = (long long)a.B * a.Hkv;
-    return (a.kv_len && groups < 64) || (a.causal && groups < 8);
+    return a.kv_len || (a.causal && (long long)a.B * a.Hkv < 16);
 }
 unsigned grid_of(const DiffArgs& a, int nx) {
     const long long n = (long long)a.B * a.Hkv * nx;

@@ -5,8 +5,9 @@
 //
 // Angles: position x turns per position in 64 bits, the whole turns taken off there, cos / sin of the rest in f32 -- exact to f32 for
 // any int32 position, where an f32 product is off by 1e-2 rad at position 1e5.  The angles of a token are the same for all its heads:
-// a block takes ROPE_TOK tokens, puts their pairs' (cos, sin) into LDS once and turns all heads from there.
-// HBM-bound: every element is read once and written once, 16 bytes a lane.
+// a block takes up to ROPE_TOK tokens, puts their pairs' (cos, sin) into LDS once and turns all heads from there.
+// HBM-bound: every element is read once and written once, 16 bytes a lane: 32 x 1568 tokens x 24 heads in bf16 57 us of graph time,
+// 5.4 TB/s; below some thousand tokens it is the launch, 3 us of GPU time and 9 of the host's.
 #include "common.h"
 #include "../../include/mofo_hip.h"
 
@@ -169,7 +170,10 @@ extern "C" int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, 
     a.gh = grid_h;
     a.gw = grid_w;
     a.in_place = x == out;
-    a.tok_per_block = M >= 8192 ? 8 : M >= 2048 ? 4 : 1;
+    // few tokens: one a block, to fill the card (160 tokens x 24 heads in bf16, us by tokens a block: 1 3.1, 4 3.7, 8 4.2; 2048 4.5, 4.6, 5.0);
+    // many: several, for the angles' share of a block's time (8192 12.4, 9.7, 9.8; 50176 76, 57, 58), more of them if their rows are short
+    // (50176 x 3 heads 39, 15, 13; 14997 x 7 heads in f32: 4 11.7, 8 11.2)
+    a.tok_per_block = M < 2048 ? 1 : W * (x_is_bf16 ? 2 : 4) >= 2048 ? ROPE_TOK / 2 : ROPE_TOK;
     hipStream_t s = (hipStream_t)stream;
     if (x_is_bf16) {
         if (interleaved) launch<true, true>(a, inverse, s);
