@@ -198,29 +198,34 @@ __device__ const u32x4 g_zero = {0, 0, 0, 0};
 struct HalfTile {
     const bf16_t* base;     // first row's 64 columns
     size_t ld;
-    int voff[2];            // byte offset of the lane's 16 bytes inside an even / odd piece (the swizzle sits on the source column)
+    int voff[2];            // byte offset of the lane's 16 bytes inside the first / second piece of 8 rows (the swizzle sits on the source column)
 };
 __device__ __forceinline__ HalfTile half_tile(const bf16_t* base, size_t ld, int lane) {
     HalfTile t;
     t.base = base;
     t.ld = ld;
 #pragma unroll
-    for (int o = 0; o < 2; ++o) t.voff[o] = (int)(((size_t)(lane >> 3) * ld + (((lane & 7) ^ swz(8 * o + (lane >> 3))) << 3)) * 2);
+    for (int o = 0; o < 2; ++o) t.voff[o] = (int)(((size_t)(8 * o + (lane >> 3)) * ld + (((lane & 7) ^ swz(8 * o + (lane >> 3))) << 3)) * 2);
     return t;
 }
-__device__ __forceinline__ void dma_piece(const void* sbase, int voff, unsigned lds_dst) {
+// Four pieces, 1 KiB each; the third and fourth lie 16 rows (p1) behind the first two.  One block: a scalar base that a vector instruction
+// wrote may be read five states later, M0 one state after it is written.
+__device__ __forceinline__ void dma_pieces(const void* p0, const void* p1, int v0, int v1, unsigned lds_dst) {
     unsigned keep;
-    asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(voff), "s"(sbase), "s"(lds_dst)
-                 : "memory");
+    asm volatile(
+        "s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\t"
+        "s_add_u32 m0, %5, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
+        "s_add_u32 m0, %5, 0x800\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %2\n\t"
+        "s_add_u32 m0, %5, 0xc00\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %2\n\ts_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "s"(p0), "s"(p1), "v"(v0), "v"(v1), "s"(lds_dst)
+        : "memory", "scc");
 }
 // rows in front of `first` and at and behind `rows` are zero
 __device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane, int first = 0) {
     if (row0 >= first && row0 + 32 <= rows) {
         const char* p = (const char*)(t.base + (size_t)row0 * t.ld);
-#pragma unroll
-        for (int sub = 0; sub < 4; ++sub) dma_piece(p + (size_t)sub * 16 * t.ld, t.voff[sub & 1], lds_dst + sub * 1024);
+        dma_pieces(p, p + t.ld * 32, t.voff[0], t.voff[1], lds_dst);
     } else {
         asm volatile("" : "+v"(lane));     // nothing of this path is to be kept in registers across a tile loop
 #pragma unroll
