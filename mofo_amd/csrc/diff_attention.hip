@@ -222,18 +222,38 @@ __device__ __forceinline__ void dma_pieces(const void* p0, const void* p1, int v
         : "memory", "scc");
 }
 // rows in front of `first` and at and behind `rows` are zero
-__device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane, int first = 0) {
-    if (row0 >= first && row0 + 32 <= rows) {
-        const char* p = (const char*)(t.base + (size_t)row0 * t.ld);
-        dma_pieces(p, p + t.ld * 32, t.voff[0], t.voff[1], lds_dst);
-    } else {
-        asm volatile("" : "+v"(lane));     // nothing of this path is to be kept in registers across a tile loop
+__device__ __forceinline__ void dma_edge(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane, int first) {
+    asm volatile("" : "+v"(lane));         // nothing of this path is to be kept in registers across a tile loop
 #pragma unroll
-        for (int sub = 0; sub < 4; ++sub) {
-            const int rl = 8 * sub + (lane >> 3), row = row0 + rl;
-            const void* src = row >= first && row < rows ? (const void*)(t.base + (size_t)row * t.ld + (((lane & 7) ^ swz(rl)) << 3)) : (const void*)&g_zero;
-            dma_b128(src, lds_dst + sub * 1024);
-        }
+    for (int sub = 0; sub < 4; ++sub) {
+        const int rl = 8 * sub + (lane >> 3), row = row0 + rl;
+        const void* src = row >= first && row < rows ? (const void*)(t.base + (size_t)row * t.ld + (((lane & 7) ^ swz(rl)) << 3)) : (const void*)&g_zero;
+        dma_b128(src, lds_dst + sub * 1024);
+    }
+}
+__device__ __forceinline__ void dma_inside(const HalfTile& t, int row0, unsigned lds_dst) {
+    const bf16_t* p = t.base + (size_t)row0 * t.ld;
+    dma_pieces(p, p + t.ld * 16, t.voff[0], t.voff[1], lds_dst);
+}
+__device__ __forceinline__ void dma_half_tile(const HalfTile& t, int row0, int rows, unsigned lds_dst, int lane, int first = 0) {
+    if (row0 >= first && row0 + 32 <= rows) dma_inside(t, row0, lds_dst);
+    else dma_edge(t, row0, rows, lds_dst, lane, first);
+}
+// both halves of a 128-wide row, of two tensors: four half tiles
+__device__ __forceinline__ void dma_tiles(HalfTile x, HalfTile y, int row0, int rows, unsigned lds_dst, int lane, int first = 0) {
+    HalfTile x1 = x, y1 = y;
+    x1.base += 64;
+    y1.base += 64;
+    if (row0 >= first && row0 + 32 <= rows) {
+        dma_inside(x, row0, lds_dst);
+        dma_inside(x1, row0, lds_dst + TILE);
+        dma_inside(y, row0, lds_dst + 2 * TILE);
+        dma_inside(y1, row0, lds_dst + 3 * TILE);
+    } else {
+        dma_edge(x, row0, rows, lds_dst, lane, first);
+        dma_edge(x1, row0, rows, lds_dst + TILE, lane, first);
+        dma_edge(y, row0, rows, lds_dst + 2 * TILE, lane, first);
+        dma_edge(y1, row0, rows, lds_dst + 3 * TILE, lane, first);
     }
 }
 // own pieces but the N newest have landed, own LDS reads are done; then every wave's
@@ -328,14 +348,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
         const int row0 = (first + t * stride) * 32;
         const unsigned at = lds0 + ring + buf * STAGE;
         if constexpr (KEYS4) {
-            HalfTile hi = ht;
-            dma_half_tile(hi, row0, len, at, lane);
-            hi.base += 64;
-            dma_half_tile(hi, row0, len, at + TILE, lane);
-            hi = hv;
-            dma_half_tile(hi, row0, len, at + 2 * TILE, lane);
-            hi.base += 64;
-            dma_half_tile(hi, row0, len, at + 3 * TILE, lane);
+            dma_tiles(ht, hv, row0, len, at, lane);
         } else {
             dma_half_tile(ht, row0, len, at + wave * TILE, lane);
         }
@@ -887,14 +900,7 @@ __device__ __forceinline__ void dq_block(int id, unsigned char* smem) {
         const int row0 = (first + t * stride) * 32;
         const unsigned at = lds0 + ring + buf * STAGE;
         if constexpr (KEYS4) {
-            HalfTile hi = ht;
-            dma_half_tile(hi, row0, len, at, lane);
-            hi.base += 64;
-            dma_half_tile(hi, row0, len, at + TILE, lane);
-            hi = hv;
-            dma_half_tile(hi, row0, len, at + 2 * TILE, lane);
-            hi.base += 64;
-            dma_half_tile(hi, row0, len, at + 3 * TILE, lane);
+            dma_tiles(ht, hv, row0, len, at, lane);
         } else {
             dma_half_tile(ht, row0, len, at + wave * TILE, lane);
         }
@@ -1092,14 +1098,9 @@ __device__ __forceinline__ void dkv_block(int id, unsigned char* smem) {
         HalfTile hi = ht;
         hi.base += (size_t)h * HV;
         if constexpr (ROWS4) {
-            dma_half_tile(hi, qt * 32, a.Nq, at, lane, row_first);
-            hi.base += 64;
-            dma_half_tile(hi, qt * 32, a.Nq, at + TILE, lane, row_first);
-            hi = ho;
-            hi.base += (size_t)h * HV;
-            dma_half_tile(hi, qt * 32, a.Nq, at + 2 * TILE, lane, row_first);
-            hi.base += 64;
-            dma_half_tile(hi, qt * 32, a.Nq, at + 3 * TILE, lane, row_first);
+            HalfTile yi = ho;
+            yi.base += (size_t)h * HV;
+            dma_tiles(hi, yi, qt * 32, a.Nq, at, lane, row_first);
         } else {
             hi.base += (wave & 1) * 64;
             dma_half_tile(hi, qt * 32, a.Nq, at + wave * TILE, lane, row_first);
