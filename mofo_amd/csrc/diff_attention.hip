@@ -313,9 +313,9 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // One block: four waves of 32 rows that share the key tiles of one (clip, key head), two tiles a barrier in a ring of four filled by LDS-DMA;
 // or KEYS4.  nsplit > 1: of a range of the keys, joined by diff_join_kernel.
 // 24 matrix instructions (768 cycles of the matrix unit) and about 150 others, 32 of them exponentials at twice the time (740 cycles), stand
-// against 2100 cycles a tile and wave that a full card takes: matrix unit 36 % and vector unit 40 % busy, LDS 17 %, two waves a SIMD (the
-// registers allow no third) whose phases meet too often.  16 clips x 6 heads x 1568 tokens 208 us, 580 TFLOP/s; one clip of 12544 890 us,
-// 543 TFLOP/s; one clip of 1568 31 us.  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
+// against the 1850 cycles a tile that a SIMD takes: matrix unit 39 % and vector unit 45 % busy, LDS 15 %, two waves a SIMD (the
+// registers allow no third) whose phases meet too often, at the 1.9 to 2.1 GHz that the card holds.  16 clips x 6 heads x 1568 tokens
+// 208 us, 580 TFLOP/s; one clip of 12544 850 us, 570 TFLOP/s; one clip of 1568 29 us.  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
 // without gain: the two maps' first products in turn, the next tile's first fragments ahead of the barrier, fences that
 // interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the register file.
 template <bool KEYS4, bool SAVE, bool SPLIT>
@@ -636,33 +636,47 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 }
 
 // joins the ranges of a row: one wave a row, lanes 0..31 the first map's 128 columns, lanes 32..63 the second's; the ranges' weights are
-// exp2(lse_range - lse), lane s holding range s.  Eight loads in flight a lane: one token against 16 caches of 8192, 8 ranges, 3 us of 32.
+// exp2(lse_range - lse), lane s of a half holding ranges s and s + 32.  A chain of latencies: the first sixteen ranges' loads go out before
+// anything is waited for (one token against 16 caches of 8192, 16 ranges: 5.5 us, 6.5 in rounds of eight behind the weights).
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, int nsplit) {
-    const int lane = threadIdx.x & 63, m = lane >> 5, d = (lane & 31) * 4;
+    constexpr int AT_ONCE = 16;
+    const int lane = threadIdx.x & 63, m = lane >> 5, sl = lane & 31, d = sl * 4;
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (size_t)a.B * a.H * a.Nq;
     if (row >= rows) return;
+    const float* pl = f.part_lse + row * nsplit * 2 + m;
+    const float v0 = sl < nsplit ? pl[2 * sl] : -__builtin_inff(), v1 = sl + 32 < nsplit ? pl[2 * (sl + 32)] : -__builtin_inff();
+    const float* pp = f.part + row * nsplit * (2 * HV) + m * HV + d;
+    f32x4 x[AT_ONCE];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) x[j] = *(const f32x4*)(pp + (size_t)min(s0 + j, nsplit - 1) * (2 * HV));
+    };
+    fetch(0);
     const size_t bh = row / a.Nq;
     const int i = (int)(row - bh * a.Nq), b = (int)(bh / a.H), h = (int)(bh - (size_t)b * a.H);
+    f32x4 gam = {1.f, 1.f, 1.f, 1.f};
+    if (a.gamma) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) gam[e] = param(a.gamma, a.param_bf16, d + e);
+    }
     float e1, e2;
     const float lam = head_lambda(a, h, lane, e1, e2);
-    float wgt[2], lse[2];
+    float top = fmaxf(v0 != v0 ? __builtin_inff() : v0, v1 != v1 ? __builtin_inff() : v1);        // a NaN of any range makes the row NaN
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const float x = lane < nsplit ? f.part_lse[(row * nsplit + lane) * 2 + n] : -__builtin_inff();
-        const float top = wave_max(x), e = top == -__builtin_inff() ? 0.f : fast_exp2(x - top), sum = wave_sum(e);
-        wgt[n] = sum > 0.f || sum != sum ? e / sum : 0.f;
-        lse[n] = sum > 0.f || sum != sum ? top + fast_log2(sum) : EMPTY_LSE;
-    }
-    const float* pp = f.part + row * nsplit * (2 * HV) + m * HV + d;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const bool none = top == -__builtin_inff();
+    float w0 = none ? 0.f : fast_exp2(v0 - top), w1 = none ? 0.f : fast_exp2(v1 - top), sum = w0 + w1;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const float lse = none ? EMPTY_LSE : top + fast_log2(sum), inv = none ? 0.f : 1.0f / sum;
+    w0 *= inv;
+    w1 *= inv;
     f32x4 acc = {0, 0, 0, 0};
-    for (int s0 = 0; s0 < nsplit; s0 += 8) {              // eight loads in flight
-        f32x4 x[8];
+    for (int s0 = 0; s0 < nsplit; s0 += AT_ONCE) {
+        if (s0) fetch(s0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = *(const f32x4*)(pp + (size_t)min(s0 + j, nsplit - 1) * (2 * HV));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // lane s holds range s's weight of both maps; ranges behind the last have none
-            const float w0 = __shfl(wgt[0], s0 + j, 64), w1 = __shfl(wgt[1], s0 + j, 64), w = m ? w1 : w0;
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const float w = __shfl(s0 < 32 ? w0 : w1, (lane & 32) + ((s0 + j) & 31), 64);      // ranges behind the last have none
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] += w != 0.f ? w * x[j][e] : 0.f;
         }
@@ -681,15 +695,13 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
     for (int x = 16; x > 0; x >>= 1) ss += __shfl_xor(ss, x, 64);
     const size_t at = ((size_t)b * a.Nq + i), off = at * a.H * HV + (size_t)h * HV + d;
     if (f.o && m) *(u32x2*)(f.o2 + off) = u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+    if (f.o && sl == 0) f.lse2[(size_t)m * rows + row] = lse;
     if (m) return;
-    if (f.o) {
-        *(u32x2*)(f.o + off) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-        if (lane < 2) f.lse2[(size_t)lane * rows + row] = lane ? lse[1] : lse[0];
-    }
+    if (f.o) *(u32x2*)(f.o + off) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
     if (a.gamma) {
         const float rn = a.out_scale / sqrtf(ss * (1.f / HV) + a.eps);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= rn * param(a.gamma, a.param_bf16, d + e);
+        for (int e = 0; e < 4; ++e) o[e] *= rn * gam[e];
     }
     *(u32x2*)(f.out + at * f.ldo + (size_t)h * HV + d) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
 }
@@ -1381,7 +1393,7 @@ bool four_way(long long groups, long long rows, long long tiles, bool causal) {
     return block_time(true, groups * ((rows + 31) / 32), tiles, causal) < block_time(false, groups * ((rows + 127) / 128), tiles, causal);
 }
 
-// Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 3 us and a
+// Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 3 us more and a
 // little per range, and a partial row is written and read at about 1500 rows a us.  At most 64 ranges and 65536 partial rows.  us by
 // ranges: one token against 16 caches of 8192 1 96, 4 36, 8 32, 16 32, 32 36; against one 1 91, 8 21, 32 16, 64 18; 11 rows x 1700 keys x
 // 36 heads 1 27, 6 17, 16 23; one head x 1568 1 24, 4 20, 8 22.

@@ -448,6 +448,21 @@ def test_diff_attention_ends_of_the_scale(dev, scale):
     assert not got["out"][N:N + 40].any() and not got["dq"][N:N + 40].any() and not got["dk"][N + 30:].any() and not got["dv"][N + 30:].any()
 
 
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv", [(2, 1, 4000, 4, 2), (1, 50, 50, 2, 1), (24, 140, 140, 12, 12)])
+def test_diff_attention_a_bad_query_stays_in_its_row(dev, B, Nq, Nk, H, Hkv):
+    """NaN in one visible query row of one head: that row is NaN in that head, in every form of the forward pass, and no other number moves"""
+    q, k, v, lam, gamma, _ = _case(dev, B, Nq, Nk, H, Hkv, True)
+    args = lambda t: (t, k, v, B, H, Hkv, 0.125, lam, 0.4, gamma, 0.6, None, 0)  # noqa: E731
+    want = _call(*args(q))["out"]
+    q2, row = q.clone(), Nq * B - 1
+    q2[row, 128 + 70] = math.nan
+    got = _call(*args(q2))["out"]
+    assert bool(torch.isnan(got[row, 128:256]).all())
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[row, 128:256] = False
+    assert torch.equal(got[same], want[same])
+
+
 def test_diff_attention_gradients_against_differences(dev):
     """the kernels' gradients along a direction against central differences of the definition in 64 bits"""
     B, N, H, Hkv = 2, 37, 4, 2
