@@ -33,6 +33,7 @@ struct DiffArgs {
     const bf16_t *q, *k, *v;
     size_t ldq, ldk, ldv;
     int B, H, Hkv, G, Nq, Nk, R, causal;
+    int row0;                 // forward and dQ: the launch's first row of every list
     const int* kv_len;
     const void* lam;          // [4][lam_heads][64]
     const void* gamma;        // [128] or NULL
@@ -315,8 +316,10 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // 24 matrix instructions (768 cycles of the matrix unit) and about 150 others, 32 of them exponentials at twice the time (740 cycles), stand
 // against the 1850 cycles a tile that a SIMD takes: matrix unit 39 % and vector unit 45 % busy, LDS 15 %, two waves a SIMD (the
 // registers allow no third) whose phases meet too often, at the 1.9 to 2.1 GHz that the card holds.  16 clips x 6 heads x 1568 tokens
-// 208 us, 580 TFLOP/s; one clip of 12544 850 us, 570 TFLOP/s; one clip of 1568 29 us.  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
-// without gain: the two maps' first products in turn, the next tile's first fragments ahead of the barrier, fences that
+// 208 us, 580 TFLOP/s; one clip of 12544 750 us, 645 TFLOP/s; one clip of 1568 29 us.  (FLOP as the formula has them, 512 a row and key; each
+// map's own second product makes 768 of it, since neither sum is known before the last key: 16 x 6 x 2048, whose blocks fill three rounds,
+// runs at 680, that is 1020 TFLOP/s of matrix work, 85 % of a large library product's rate.)  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
+// without gain: blocks of eight waves whose two halves do products and softmax in opposite phases, a barrier between; the two maps' first products in turn, the next tile's first fragments ahead of the barrier, fences that
 // interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the register file.
 template <bool KEYS4, bool SAVE, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
     if (!place_block(a, blockIdx.x, nx * nsplit, spread, true, xs, b, kvh)) return;
     const int xb = xs / nsplit, sp = xs - xb * nsplit;
     const int len = clip_len(a, b);
-    const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
+    const int rb0 = a.row0 + xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
     span_lim(a, len, rb0, min(rb0 + ROWS, a.R) - 1, blo, bhi);
@@ -897,7 +900,7 @@ __device__ __forceinline__ void dq_block(int id, unsigned char* smem) {
     int xb, b, kvh;
     if (!place_block(a, id, in.nxq, in.spread, true, xb, b, kvh)) return;
     const int len = clip_len(a, b);
-    const int rb0 = xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
+    const int rb0 = a.row0 + xb * ROWS, r0 = rb0 + (KEYS4 ? 0 : wave * 32);
     const Row w = make_row(a, kvh, r0 + (lane & 31), len);
     int wlo = 0, whi = 0, blo, bhi;
     span_lim(a, len, rb0, min(rb0 + ROWS, a.R) - 1, blo, bhi);
@@ -1358,6 +1361,7 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
     a.Nk = Nk;
     a.R = a.G * Nq;
     a.causal = causal;
+    a.row0 = 0;
     a.kv_len = kv_len;
     a.lam = lam;
     a.gamma = gamma;
@@ -1392,6 +1396,21 @@ double block_time(bool four, long long blocks, long long tiles, bool causal) {
 bool four_way(long long groups, long long rows, long long tiles, bool causal) {
     return block_time(true, groups * ((rows + 31) / 32), tiles, causal) < block_time(false, groups * ((rows + 127) / 128), tiles, causal);
 }
+// Equal blocks, `others` of another part in front of them: beyond 512 the rows of the last, partial round may be left to four-way blocks in
+// a launch behind the first.  nx 128-row blocks a list.  us, all rows in 128-row blocks, in four-way ones, and 85 blocks and 52 four-way ones
+// a list: forward 6 heads x 12544 890 / 848 / 746.
+struct Cut {
+    long long nx;
+    double time;
+};
+Cut cut_rows(long long others, long long groups, long long rows, long long tiles) {
+    const long long n = (rows + 127) / 128, full = (others + groups * n) / 512 * 512 - others, nx = full > 0 ? full / groups : 0;
+    const double whole = block_time(false, others + groups * n, tiles, false);
+    if (nx <= 0 || nx >= n) return {n, whole};
+    const double cut = block_time(false, others + groups * nx, tiles, false) + block_time(true, groups * ((rows - nx * 128 + 31) / 32), tiles, false) + 3.0;
+    return cut < whole ? Cut{nx, cut} : Cut{n, whole};
+}
+int tail_blocks(const Cut& c, long long rows) { return c.nx * 128 < rows ? (int)((rows - c.nx * 128 + 31) / 32) : 0; }
 
 // Forward: four-way blocks may cut the keys into ranges as well (few rows against a long cache), joined by a kernel of its own: 3 us more and a
 // little per range, and a partial row is written and read at about 1500 rows a us.  At most 64 ranges and 65536 partial rows.  us by
@@ -1399,19 +1418,20 @@ bool four_way(long long groups, long long rows, long long tiles, bool causal) {
 // 36 heads 1 27, 6 17, 16 23; one head x 1568 1 24, 4 20, 8 22.
 struct FwdPlan {
     bool keys4;
-    int nx, nsplit;
+    int nx, nsplit, tail;     // tail: four-way blocks a list behind nx * 128 rows, in a launch of their own
 };
 FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv, int causal) {
     const long long R = (long long)(H / Hkv) * Nq, rows = (long long)B * H * Nq, groups = (long long)B * Hkv, tiles = (Nk + 31) / 32;
     const long long n1 = (R + 127) / 128, n4 = (R + 31) / 32;
     const bool half = causal == 1;                        // towards the end: every row sees nearly all keys
-    FwdPlan p = {false, (int)n1, 1};
-    double best = block_time(false, groups * n1, tiles, half);
+    const Cut c = half ? Cut{n1, block_time(false, groups * n1, tiles, true)} : cut_rows(0, groups, R, tiles);
+    FwdPlan p = {false, (int)c.nx, 1, tail_blocks(c, R)};
+    double best = c.time;
     for (int n = 1; n <= 64 && (n == 1 || (n <= tiles && n * rows <= 65536)); ++n) {
         const double t = block_time(true, groups * n4 * n, (tiles + n - 1) / n, half) + (n > 1 ? 3.0 + 0.05 * n + n * rows / 1500.0 : 0.0);
         if (t < best) {
             best = t;
-            p = {true, (int)n4, n};
+            p = {true, (int)n4, n, 0};
         }
     }
     return p;
@@ -1459,7 +1479,7 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
                                {"gamma", gamma, 1, HV * es, 0}, {"kv_len", kv_len, 1, 4LL * B, 0}};
         MOFO_CHECK_APART("mofo_diff_attention_fwd", outs, 5, in, 6);
     }
-    const DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
+    DiffArgs a = make_args(q, ldq, k, ldk, v, ldv, B, Nq, Nk, H, Hkv, scale, lam, lam_heads, lam_init, gamma, param_is_bf16, eps, out_scale, kv_len, causal);
     FwdOut f = {(bf16_t*)out, (bf16_t*)o, (bf16_t*)o2, (size_t)ldo, lse2, nullptr, nullptr};
     if (pl.nsplit > 1) {
         f.part = ws;
@@ -1468,15 +1488,24 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
     const int spread = spread_of(a);
     const dim3 grid(grid_of(a, pl.nx * pl.nsplit));
     hipStream_t s = (hipStream_t)stream;
+    auto four_way_rows = [&](int nx) {
+        const dim3 g(grid_of(a, nx));
+        if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, false>), g, dim3(256), 0, s, a, f, nx, 1, spread);
+        else hipLaunchKernelGGL((diff_fwd_kernel<true, false, false>), g, dim3(256), 0, s, a, f, nx, 1, spread);
+    };
     if (pl.nsplit > 1) {
         if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, true>), grid, dim3(256), 0, s, a, f, pl.nx, pl.nsplit, spread);
         else hipLaunchKernelGGL((diff_fwd_kernel<true, false, true>), grid, dim3(256), 0, s, a, f, pl.nx, pl.nsplit, spread);
     } else if (pl.keys4) {
-        if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
-        else hipLaunchKernelGGL((diff_fwd_kernel<true, false, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+        four_way_rows(pl.nx);
     } else {
         if (o) hipLaunchKernelGGL((diff_fwd_kernel<false, true, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
         else hipLaunchKernelGGL((diff_fwd_kernel<false, false, false>), grid, dim3(256), 0, s, a, f, pl.nx, 1, spread);
+    }
+    if (pl.tail) {
+        MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd");
+        a.row0 = pl.nx * 128;
+        four_way_rows(pl.tail);
     }
     MOFO_CHECK_LAUNCH("mofo_diff_attention_fwd");
     if (pl.nsplit > 1) {
@@ -1537,13 +1566,25 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
     const long long groups = (long long)B * Hkv, kt = (Nk + 31) / 32, qt = (long long)a.G * ((Nq + 31) / 32);
-    const bool q4 = four_way(groups, a.R, kt, causal == 1), k4 = four_way(groups, Nk, qt, causal != 0);
+    bool q4 = four_way(groups, a.R, kt, causal == 1), k4 = four_way(groups, Nk, qt, causal != 0);
+    Cut cut = {ceil_div(a.R, 128), 0.0};
+    if (!causal && qt == kt) {                            // equal blocks throughout: dQ's last rows may fill up the last round
+        // us, dK / dV and dQ in four-way blocks, and in 128-row blocks with a tail: 6 heads x 12544 2060 / 1822, 12 x 6000 975 / 846, 6 x 1568 65 / 76
+        const long long nk = groups * ceil_div(Nk, 128), nq = groups * cut.nx, nq4 = groups * ceil_div(a.R, 32);
+        const Cut c = cut_rows(nk, groups, a.R, kt);
+        const double chosen = q4 && k4 ? block_time(true, groups * kt + nq4, kt, false)
+                              : q4 || k4 ? block_time(k4, k4 ? groups * kt : nk, kt, false) + block_time(q4, q4 ? nq4 : nq, kt, false) : 1e30;
+        if (1.15 * c.time < chosen) {                     // a step of dK / dV is longer than the model's
+            q4 = k4 = false;
+            cut = c;
+        }
+    }
     GradArgs g = {a, dy, lddy, stats, lams, part, (bf16_t*)dq, (bf16_t*)dk, (bf16_t*)dv, (size_t)lddq, (size_t)lddk, (size_t)lddv, dlam, dgamma, nb, grad_is_bf16};
     g.params = lam_heads + (dgamma ? 16 : 0);
     g.np = (g.params + 7) / 8 * 8;
     g.nxk = ceil_div(Nk, k4 ? 32 : 128);
     g.nk = (int)grid_of(a, g.nxk);
-    g.nxq = ceil_div(a.R, q4 ? 32 : 128);
+    g.nxq = q4 ? ceil_div(a.R, 32) : (int)cut.nx;
     g.spread = spread_of(a);
     const dim3 grid(g.np + g.nk + grid_of(a, g.nxq));
     if (q4 && k4) hipLaunchKernelGGL((diff_grad_kernel<true, true>), grid, dim3(256), 0, s, g);
@@ -1551,5 +1592,13 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     else if (k4) hipLaunchKernelGGL((diff_grad_kernel<false, true>), grid, dim3(256), 0, s, g);
     else hipLaunchKernelGGL((diff_grad_kernel<false, false>), grid, dim3(256), 0, s, g);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(gradients)");
+    const int tail = q4 ? 0 : tail_blocks(cut, a.R);
+    if (tail) {
+        g.a.row0 = g.nxq * 128;
+        g.np = g.params = g.nk = 0;
+        g.nxq = tail;
+        hipLaunchKernelGGL((diff_grad_kernel<true, false>), dim3(grid_of(a, tail)), dim3(256), 0, s, g);
+        MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(last rows)");
+    }
     return MOFO_OK;
 }

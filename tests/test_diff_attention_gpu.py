@@ -331,6 +331,8 @@ MANY = [  # enough (clip, key head) pairs for blocks of 128 rows (keys) in every
     (67, 100, 100, 8, 4, 1, None, True, None, BF16),                          # two heads a key head, causal from the start
     (10, 500, 500, 8, 4, 2, (0, 500, 1, 499, 33, 128, 257, 500, 64, 129), True, None, BF16),          # ragged: one list over all XCDs
     (70, 50, 170, 4, 4, 2, tuple((b * 37) % 172 for b in range(70)), False, None, BF16),
+    (110, 544, 544, 1, 1, 0, None, True, None, BF16),                         # whole rounds of 128-row blocks, the last rows in four-way ones
+    (28, 272, 272, 8, 4, 0, tuple((b * 61) % 280 for b in range(28)), False, None, F32),
     (1, 2150, 2150, 8, 8, 1, None, True, 1, BF16)]                            # four-way, more blocks than the card holds at a time
 
 
