@@ -4,6 +4,7 @@ PyTorch is plumbing here (device memory + streams); every computation is a kerne
 These wrappers validate device / dtype / layout so that a wrong shape raises here instead of faulting on the GPU.
 """
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -525,9 +526,14 @@ def _dev_chk(dev, dtype, dims, **tensors):
 _INT4 = C.c_int * 4
 
 
-def _ld16(t):
-    """row pitch of a 2-D tensor; a single row's own stride says nothing"""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _pitch(dev, dtype, name, t):
+    """row pitch of a matrix that ``_dev_chk`` lets through (a single row's own stride says nothing)"""
+    if t is not None:
+        s = t.stride()
+        if len(s) == 2 and s[1] == 1 and t.dtype is dtype and t.get_device() == dev:
+            return s[0] if t.shape[0] > 1 else t.shape[1]
+    _chk(t, dtype, name, 2)
+    raise ValueError(f"{name} must be on the current device cuda:{dev}, it is on {t.device}")
 
 
 def rope_freqs(sections, base=10000.0, device="cuda"):
@@ -536,22 +542,30 @@ def rope_freqs(sections, base=10000.0, device="cuda"):
     return torch.tensor([base ** (-i / n) / (2 * math.pi) for n in sections for i in range(n)], dtype=torch.float64, device=device)
 
 
+@functools.lru_cache(maxsize=64)
+def _rope_sections(sections, head_dim):
+    """sum of the sections, and the sections as the library takes them"""
+    if not 1 <= len(sections) <= 4 or min(sections) < 0:
+        raise ValueError("rope_axes: one to four sections, none negative")
+    pairs = sum(sections)
+    if pairs < 8 or pairs % 8 or pairs > 128 or 2 * pairs > head_dim or head_dim % 16 or head_dim > 1024:
+        raise ValueError("rope_axes: pairs a multiple of 8 up to 128, 2 * pairs <= head_dim, head_dim a multiple of 16 up to 1024")
+    return pairs, _INT4(*sections)
+
+
 def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, interleaved, inverse, nx, nout):
     if x is None or x.dtype not in (F32, BF16):
         raise TypeError(f"{nx} must be f32 or bf16")
     dt, dev = x.dtype, torch.cuda.current_device() if x.is_cuda else -1
-    _dev_chk(dev, dt, 2, **{nx: x, nout: out})
+    if dev < 0 or freqs is None:
+        _chk(x, dt, nx), _chk(freqs, torch.float64, "freqs")
+    ldx, ldo = _pitch(dev, dt, nx, x), _pitch(dev, dt, nout, out)
     _dev_chk(dev, torch.float64, 1, freqs=freqs)
-    if not x.is_cuda or out is None or freqs is None:
-        _chk(x, dt, nx), _chk(out, dt, nout), _chk(freqs, torch.float64, "freqs")
-    M, axes = x.shape[0], len(sections)
-    if not 1 <= axes <= 4 or min(sections) < 0:
-        raise ValueError("rope_axes: one to four sections, none negative")
-    pairs = sum(sections)
-    if x.shape[1] != heads * head_dim or out.shape != x.shape:
+    shape, axes = x.shape, len(sections)
+    M = shape[0]
+    pairs, sections = _rope_sections(tuple(sections), head_dim)
+    if shape[1] != heads * head_dim or out.shape != shape:
         raise ValueError(f"rope_axes: {nx} and {nout} must be [M, heads * head_dim]")
-    if pairs < 8 or pairs % 8 or pairs > 128 or 2 * pairs > head_dim or head_dim % 16 or head_dim > 1024:
-        raise ValueError("rope_axes: pairs a multiple of 8 up to 128, 2 * pairs <= head_dim, head_dim a multiple of 16 up to 1024")
     if freqs.shape[0] != pairs:
         raise ValueError("rope_axes: freqs must hold one value a pair")
     if (pos is None) == (tok_idx is None):
@@ -567,8 +581,8 @@ def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, int
             raise ValueError("rope_axes: tok_idx must hold M contiguous ids, with three sections and a grid (T, H, W)")
         gh, gw = grid[1], grid[2]
     if M:
-        _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), x.data_ptr(), 1 if dt is BF16 else 0, _ld16(x), out.data_ptr(), _ld16(out), M,
-             heads, head_dim, freqs.data_ptr(), axes, _INT4(*sections), _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
+        _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), x.data_ptr(), 1 if dt is BF16 else 0, ldx, out.data_ptr(), ldo, M,
+             heads, head_dim, freqs.data_ptr(), axes, sections, _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)
     return out
 
 
@@ -602,19 +616,21 @@ def diff_attention_bwd_ws(B, Nq, Nk, H, Hkv, norm):
 
 
 def _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws):
-    """types and shapes that forward and gradient share -> (device, Nq, Nk)"""
-    for name, t in (("q", q), ("k", k), ("v", v), ("lam", lam)):
-        if t is None or not t.is_cuda:
-            _chk(t, BF16, name)
+    """types and shapes that forward and gradient share -> (device, Nq, Nk, row pitches of q, k, v)"""
+    if q is None or lam is None or not q.is_cuda or not lam.is_cuda:
+        _chk(q, BF16, "q"), _chk(lam, BF16, "lam")
     dev = torch.cuda.current_device()
     pt = lam.dtype
     if pt is not BF16 and pt is not F32:
         raise TypeError(f"{who}: lam must be f32 or bf16")
-    _dev_chk(dev, BF16, 2, q=q, k=k, v=v)
+    pitches = _pitch(dev, BF16, "q", q), _pitch(dev, BF16, "k", k), _pitch(dev, BF16, "v", v)
     _dev_chk(dev, pt, 3, lam=lam)
-    _dev_chk(dev, pt, 1, gamma=gamma)
-    _dev_chk(dev, I32, 1, kv_len=kv_len)
-    _dev_chk(dev, F32, 1, ws=ws)
+    if gamma is not None:
+        _dev_chk(dev, pt, 1, gamma=gamma)
+    if kv_len is not None:
+        _dev_chk(dev, I32, 1, kv_len=kv_len)
+    if ws is not None:
+        _dev_chk(dev, F32, 1, ws=ws)
     (Mq, Wq), (Mk, Wk) = q.shape, k.shape
     if B <= 0 or H <= 0 or Hkv <= 0 or H % Hkv or Mq % B or Mk % B:
         raise ValueError(f"{who}: B clips of the same number of rows, H a multiple of Hkv")
@@ -629,7 +645,7 @@ def _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws):
         raise ValueError(f"{who}: kv_len must have B entries")
     if causal not in (0, 1, 2):
         raise ValueError(f"{who}: causal must be 0, 1 (from the start) or 2 (towards the end)")
-    return dev, Mq // B, Mk // B
+    return dev, Mq // B, Mk // B, pitches
 
 
 def _diff_saved(who, dev, saved, B, Nq, H):
@@ -653,16 +669,16 @@ def diff_attention_fwd(q, k, v, B, H, Hkv, scale, lam, lam_init, out, gamma=None
     ``kv_len`` i32 [B]: keys each clip holds; ``causal`` 1: key <= query, 2: the queries are the last Nq of the clip's keys.  A row that sees
     no key gives zeros.  ``scale`` 2^-24 .. 2^24, ``eps`` at least 2^-100.  ``saved`` = (o, o2, lse2): kept for ``diff_attention_bwd``.
     ``ws``: f32, diff_attention_fwd_ws elements."""
-    dev, Nq, Nk = _diff_chk("diff_attention_fwd", q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
-    _dev_chk(dev, BF16, 2, out=out)
-    if out is None or out.shape != q.shape:
+    dev, Nq, Nk, (ldq, ldk, ldv) = _diff_chk("diff_attention_fwd", q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
+    ldo = _pitch(dev, BF16, "out", out)
+    if out.shape != q.shape:
         raise ValueError("diff_attention_fwd: out must have q's shape")
     o = o2 = lse2 = None
     if saved is not None:
         o, o2, lse2 = _diff_saved("diff_attention_fwd", dev, saved, B, Nq, H)
-    _run("mofo_diff_attention_fwd", ("diff_attn_fwd",), 512.0 * B * H * Nq * Nk, q.data_ptr(), _ld16(q), k.data_ptr(), _ld16(k), v.data_ptr(), _ld16(v), B, Nq,
+    _run("mofo_diff_attention_fwd", ("diff_attn_fwd",), 512.0 * B * H * Nq * Nk, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, B, Nq,
          Nk, H, Hkv, scale, lam.data_ptr(), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype is BF16 else 0, eps, out_scale, _p(kv_len), causal,
-         out.data_ptr(), _ld16(out), _p(o), _p(o2), _p(lse2), _p(ws), 0 if ws is None else ws.numel())
+         out.data_ptr(), ldo, _p(o), _p(o2), _p(lse2), _p(ws), 0 if ws is None else ws.numel())
     return out
 
 
@@ -671,10 +687,10 @@ def diff_attention_bwd(q, k, v, B, H, Hkv, scale, lam, lam_init, saved, dout, dq
     """every gradient of ``diff_attention_fwd`` (same arguments, its ``saved``), overwritten: ``dq``, ``dk``, ``dv`` bf16 like q, k, v, ``dlam`` (and
     ``dgamma``) f32 or bf16 like lam (gamma).  ``ws``: f32, diff_attention_bwd_ws elements."""
     who = "diff_attention_bwd"
-    dev, Nq, Nk = _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
+    dev, Nq, Nk, (ldq, ldk, ldv) = _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
     o, o2, lse2 = _diff_saved(who, dev, saved, B, Nq, H)
-    _dev_chk(dev, BF16, 2, dout=dout, dq=dq, dk=dk, dv=dv)
-    if dout is None or dq is None or dk is None or dv is None or dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
+    lddo, lddq, lddk, lddv = _pitch(dev, BF16, "dout", dout), _pitch(dev, BF16, "dq", dq), _pitch(dev, BF16, "dk", dk), _pitch(dev, BF16, "dv", dv)
+    if dout.shape != q.shape or dq.shape != q.shape or dk.shape != k.shape or dv.shape != k.shape:
         raise ValueError(f"{who}: dout and dq like q, dk and dv like k")
     if dlam is None or dlam.dtype not in (F32, BF16):
         raise TypeError(f"{who}: dlam must be f32 or bf16")
@@ -687,10 +703,10 @@ def diff_attention_bwd(q, k, v, B, H, Hkv, scale, lam, lam_init, saved, dout, dq
         raise ValueError(f"{who}: gamma and dgamma go together, 128 entries each")
     if ws is None:
         raise ValueError(f"{who}: ws must hold diff_attention_bwd_ws floats")
-    _run("mofo_diff_attention_bwd", ("diff_attn_bwd",), 1024.0 * B * H * Nq * Nk, q.data_ptr(), _ld16(q), k.data_ptr(), _ld16(k), v.data_ptr(), _ld16(v), B, Nq,
+    _run("mofo_diff_attention_bwd", ("diff_attn_bwd",), 1024.0 * B * H * Nq * Nk, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, B, Nq,
          Nk, H, Hkv, scale, lam.data_ptr(), lam.shape[1], lam_init, _p(gamma), 1 if lam.dtype is BF16 else 0, eps, out_scale, _p(kv_len), causal,
-         o.data_ptr(), o2.data_ptr(), lse2.data_ptr(), dout.data_ptr(), _ld16(dout), dq.data_ptr(), _ld16(dq), dk.data_ptr(), _ld16(dk), dv.data_ptr(),
-         _ld16(dv), dlam.data_ptr(), _p(dgamma), 1 if gt is BF16 else 0, ws.data_ptr(), ws.numel())
+         o.data_ptr(), o2.data_ptr(), lse2.data_ptr(), dout.data_ptr(), lddo, dq.data_ptr(), lddq, dk.data_ptr(), lddk, dv.data_ptr(),
+         lddv, dlam.data_ptr(), _p(dgamma), 1 if gt is BF16 else 0, ws.data_ptr(), ws.numel())
 
 
 def mask_to_indices(mask_u8, n_vis, vis_idx, msk_idx, status):
