@@ -316,11 +316,13 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // 24 matrix instructions (768 cycles of the matrix unit) and about 150 others, 32 of them exponentials at twice the time (740 cycles), stand
 // against the 1850 cycles a tile that a SIMD takes: matrix unit 39 % and vector unit 45 % busy, LDS 15 %, two waves a SIMD (the
 // registers allow no third) whose phases meet too often, at the 1.9 to 2.1 GHz that the card holds.  16 clips x 6 heads x 1568 tokens
-// 208 us, 580 TFLOP/s; one clip of 12544 750 us, 645 TFLOP/s; one clip of 1568 29 us.  (FLOP as the formula has them, 512 a row and key; each
+// 209 us, 578 TFLOP/s; one clip of 12544 750 us, 645 TFLOP/s; one clip of 1568 29 us.  (FLOP as the formula has them, 512 a row and key; each
 // map's own second product makes 768 of it, since neither sum is known before the last key: 16 x 6 x 2048, whose blocks fill three rounds,
-// runs at 680, that is 1020 TFLOP/s of matrix work, 85 % of a large library product's rate.)  Without exponentials it is 7 % faster, without the second products 23 %, without loads 10 %.  Tried
-// without gain: blocks of eight waves whose two halves do products and softmax in opposite phases, a barrier between; the two maps' first products in turn, the next tile's first fragments ahead of the barrier, fences that
-// interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the register file.
+// runs at 680, that is 1020 TFLOP/s of matrix work, 85 % of a large library product's rate.)  At 1568, without exponentials it is 7 % faster,
+// without the second products 23 %, without loads 10 %.  Tried without gain: blocks of eight waves whose two halves do products and
+// softmax in opposite phases, a barrier between; the two maps' first products in turn; the next tile's first fragments ahead of the
+// barrier; fences that interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the
+// register file.
 template <bool KEYS4, bool SAVE, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, int nx, int nsplit, int spread) {
     constexpr int STAGE = 4 * TILE, ROWS = KEYS4 ? 32 : 128, XCH = 4 * STAGE;

@@ -7,7 +7,7 @@
 // any int32 position, where an f32 product is off by 1e-2 rad at position 1e5.  The angles of a token are the same for all its heads:
 // a block takes up to ROPE_TOK tokens, puts their pairs' (cos, sin) into LDS once and turns all heads from there.
 // HBM-bound: every element is read once and written once, 16 bytes a lane: 32 x 1568 tokens x 24 heads in bf16 57 us of graph time,
-// 5.4 TB/s; below some thousand tokens it is the launch, 3 us of GPU time and 9 of the host's.
+// 5.4 TB/s; below some thousand tokens it is the launch, 3 us of GPU time and 9 of the host's call.
 #include "common.h"
 #include "../../include/mofo_hip.h"
 
