@@ -120,6 +120,21 @@ def test_rope_axes_far_positions(dev):
     _within(out, want, size * (2.0 ** -20 + 2.0 ** 31 * 2.0 ** -51), "far")   # the f64 angle itself: 2^31 at 2^-52 a side
 
 
+def test_rope_axes_offsets_beyond_32_bits(dev):
+    """rows 2^20 elements apart: the last ones start behind element 2^31; in place the same bits"""
+    from mofo_amd import ops
+    M, big = 2200, torch.empty(2200, 1 << 20, dtype=BF16, device=dev)
+    x = _rand((M, 128), dev, 3)
+    big[:, 64:192] = x
+    pos, freqs = torch.arange(3 * M, dtype=I32, device=dev).reshape(M, 3), ops.rope_freqs((8, 12, 12), device=dev)
+    want, out = torch.empty_like(x), torch.empty_like(x)
+    ops.rope_axes_fwd(x, 2, 64, (8, 12, 12), freqs, want, pos=pos)
+    ops.rope_axes_fwd(big[:, 64:192], 2, 64, (8, 12, 12), freqs, out, pos=pos)
+    assert torch.equal(out, want)
+    ops.rope_axes_fwd(big[:, 64:192], 2, 64, (8, 12, 12), freqs, big[:, 64:192], pos=pos)
+    assert torch.equal(big[:, 64:192], want)
+
+
 def test_rope_axes_no_rows(dev):
     from mofo_amd import ops
     x = torch.empty(0, 64, dtype=BF16, device=dev)
@@ -333,6 +348,7 @@ MANY = [  # enough (clip, key head) pairs for blocks of 128 rows (keys) in every
     (70, 50, 170, 4, 4, 2, tuple((b * 37) % 172 for b in range(70)), False, None, BF16),
     (110, 544, 544, 1, 1, 0, None, True, None, BF16),                         # whole rounds of 128-row blocks, the last rows in four-way ones
     (28, 272, 272, 8, 4, 0, tuple((b * 61) % 280 for b in range(28)), False, None, F32),
+    (20000, 1, 3, 4, 1, 2, None, True, 1, BF16), (3, 5, 77, 64, 1, 2, (77, 4, 0), True, None, F32),   # many clips of one token, many heads on one
     (1, 2150, 2150, 8, 8, 1, None, True, 1, BF16)]                            # four-way, more blocks than the card holds at a time
 
 
