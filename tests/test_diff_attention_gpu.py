@@ -403,11 +403,11 @@ def test_diff_attention_few_tokens_against_a_cache(dev, B, Nq, Nk, H, Hkv, lens,
     _check(_call(*args, dout=dout), want)
 
 
-def test_diff_attention_masked_places_may_hold_anything(dev):
+@pytest.mark.parametrize("B,N,H,Hkv,lens", [(3, 70, 4, 2, (70, 33, 0)), (40, 140, 8, 8, tuple((b * 29) % 141 for b in range(40))), (12, 1111, 8, 2, tuple(range(0, 1200, 100)))])
+def test_diff_attention_masked_places_may_hold_anything(dev, B, N, H, Hkv, lens):
     """NaN and infinities behind kv_len in k and v, and in q and dout of rows that see nothing, reach no output and no gradient"""
-    B, N, H, Hkv = 3, 70, 4, 2
     q, k, v, lam, gamma, dout = _case(dev, B, N, N, H, Hkv, True)
-    kv_len = torch.tensor([70, 33, 0], dtype=I32, device=dev)
+    kv_len = torch.tensor(lens, dtype=I32, device=dev)
     for causal in (0, 2):
         lim = _limits(B, N, N, kv_len, causal, dev).reshape(-1)
         behind = (torch.arange(N, device=dev)[None] >= kv_len[:, None]).reshape(-1)
