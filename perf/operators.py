@@ -203,7 +203,7 @@ def _frequencies(case, dev):
 def _scratch(case):
     rows = case["B"] * case["Nq"] * case["H"]
     parts = 260 * min(64 * rows, 1 << 16)
-    return max(parts, rows * (DV // 2 + 4) + (1 << 18)) if case["op"] == "train" else parts
+    return max(parts, rows * (DV // 2 + 2) + (1 << 18)) if case["op"] == "train" else parts
 
 
 # ------------------------------------------------------------------------------------------------------------ plain form
