@@ -780,7 +780,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(DiffArgs a, const bf16_t
                 const float k = gx * rn * rn * (1.f / HV);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (mine) dg[e] += a.out_scale * vd[e] * vo[e] * rn;
+                    if (mine && some[j]) dg[e] += a.out_scale * vd[e] * vo[e] * rn;    // not 0 times whatever dout holds there
                     gg[e] = some[j] ? rn * (gg[e] - vo[e] * k) : 0.f;
                 }
 #pragma unroll

@@ -664,3 +664,23 @@ def test_diff_attention_refusals(dev):
         with pytest.raises(RuntimeError):
             bad()
     fwd()(), bwd()()
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,lens,causal", [
+    (3, 70, 70, 4, 2, (70, 33, 0), 0), (3, 70, 70, 4, 2, (0, 70, 5), 1), (3, 70, 70, 4, 2, (70, 33, 0), 2), (2, 64, 32, 4, 2, (32, 7), 2),
+    (40, 140, 140, 8, 8, tuple((b * 29) % 141 for b in range(40)), 2)])
+def test_diff_attention_gradients_of_rows_that_see_nothing_are_not_taken(dev, norm, B, Nq, Nk, H, Hkv, lens, causal):
+    """NaN and infinities in dout, and in q, of rows that see no key: every output and every gradient, dgamma among them, keeps its bits"""
+    q, k, v, lam, gamma, dout = _case(dev, B, Nq, Nk, H, Hkv, norm)
+    kv_len = torch.tensor(lens, dtype=I32, device=dev)
+    nothing = (_limits(B, Nq, Nk, kv_len, causal, dev) == 0).reshape(-1)
+    assert bool(nothing.any()) and not bool(nothing.all())
+    args = lambda t: (t, k, v, B, H, Hkv, 0.125, lam, 0.45, gamma, 0.55 if norm else 1.0, kv_len, causal)  # noqa: E731
+    want = _call(*args(q), dout=dout)
+    for bad in (math.nan, math.inf):
+        q2, d2 = q.clone(), dout.clone()
+        q2[nothing], d2[nothing] = bad, bad
+        got = _call(*args(q2), dout=d2)
+        for n in want:
+            assert torch.equal(got[n], want[n]), (n, bad)
