@@ -193,7 +193,8 @@ int mofo_attention_bwd_dq_delta_range(const void* qkv, int ldqkv, const void* ou
  * Pair i is columns (i, pairs + i) of the head, or (2 i, 2 i + 1) when interleaved; axis a owns sections[a] consecutive pairs.
  * freqs f64 [pairs]: TURNS per position (angle / 2 pi).  Places: pos i32 [M, naxes], or tok_idx i32 [M] = token ids >= 0 on a grid of
  * rows grid_h x grid_w (id = (t * grid_h + h) * grid_w + w, what mofo_mask_to_indices writes); exactly one of the two.
- * pairs a multiple of 8 up to 128, head_dim a multiple of 16 up to 1024; rows in 16-byte aligned pieces. ---- */
+ * pairs a multiple of 8 up to 128, head_dim a multiple of 16 up to 1024; rows in 16-byte aligned pieces.  At most 2^24 - 1 blocks of 4 rows
+ * (rows of 2 KiB or more) or 8 rows. ---- */
 int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, int ldo, int M, int heads, int head_dim, const double* freqs, int naxes,
                    const int* sections, const int* pos, const int* tok_idx, int grid_h, int grid_w, int interleaved, int inverse, void* stream);
 
@@ -206,7 +207,8 @@ int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, int ldo, in
  * Key j of clip b is visible to query i iff j < kv_len[b] (i32 [B]; NULL: Nk; values are cut to 0 .. Nk) and, causal = 1: j <= i;
  * causal = 2: j <= i + kv_len[b] - Nq (new tokens at the end of a cache).  A row that sees nothing gives zeros, and takes none of
  * the gradients.  Rows of k, v at and behind kv_len[b] may hold anything; rows in front of it are expected to be finite.
- * scale: 2^-24 .. 2^24; eps (with gamma): at least 2^-100.
+ * scale: 2^-24 .. 2^24; eps (with gamma): at least 2^-100.  A launch takes at most 2^24 - 1 blocks (a (clip, key head) pair's lists of 32 or 128
+ * rows, and in the gradient of keys too); calls of more are refused before anything is launched.
  * For the gradient keep o, o2 (bf16 [B * Nq, H * 128], contiguous) and lse2 (f32 [2, B, H, Nq], log2-sum-exp2); NULL all three otherwise.
  * ws: mofo_diff_attention_fwd_ws floats of scratch (0: NULL is fine), contents of no interest; two calls that may run at once (two
  * streams, two captured graphs) need one each. ---- */

@@ -35,6 +35,9 @@ void mofo_set_error(const char* fmt, ...);
         if (e__ != hipSuccess) MOFO_FAIL(MOFO_ELAUNCH, "%s: %s", name, hipGetErrorString(e__)); \
     } while (0)
 
+// A launch has fewer than 2^32 threads in x: blocks of 256 at most.
+constexpr long long MOFO_MAX_BLOCKS_256 = (1LL << 24) - 1;
+
 // A tensor as an entry sees it: `rows` rows of `cols` bytes, `ld` bytes apart.  Column ranges of one packed buffer interleave in memory
 // without sharing an element: with the same pitch, ranges that stay apart within a row do not overlap.
 struct MofoSpan {

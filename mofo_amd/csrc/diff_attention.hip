@@ -15,6 +15,7 @@
 // between the inputs and the f32 accumulators; softmax sums, statistics and norms stay f32.
 #include "common.h"
 #include "../../include/mofo_hip.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -1345,6 +1346,10 @@ int check(const char* who, const void* q, int ldq, const void* k, int ldk, const
     if ((long long)B * Hkv * (((long long)(H / Hkv) * Nq + Nk) / 32 + 2) > (1LL << 28)) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: grid too large", who);
     return MOFO_OK;
 }
+int check_blocks(const char* who, long long blocks) {
+    if (blocks > MOFO_MAX_BLOCKS_256) MOFO_FAIL(MOFO_EUNSUPPORTED, "%s: %lld blocks of a launch (at most %lld)", who, blocks, MOFO_MAX_BLOCKS_256);
+    return MOFO_OK;
+}
 
 DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, int B, int Nq, int Nk, int H, int Hkv, float scale,
                    const void* lam, int lam_heads, float lam_init, const void* gamma, int param_bf16, float eps, float out_scale, const int* kv_len, int causal) {
@@ -1445,9 +1450,9 @@ FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv, int causal) {
 int spread_of(const DiffArgs& a) {
     return a.kv_len || (a.causal && (long long)a.B * a.Hkv < 16);
 }
-unsigned grid_of(const DiffArgs& a, int nx) {
+long long grid_of(const DiffArgs& a, int nx) {
     const long long n = (long long)a.B * a.Hkv * nx;
-    return (unsigned)(8 * ((n + 7) / 8));
+    return 8 * ((n + 7) / 8);
 }
 // blocks of one head's rows in the row pass: about 1024 in all, 64 rows each at least
 int row_blocks(int B, int Nq, int H) {
@@ -1488,10 +1493,12 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
         f.part_lse = ws + rows * pl.nsplit * (2 * HV);
     }
     const int spread = spread_of(a);
-    const dim3 grid(grid_of(a, pl.nx * pl.nsplit));
+    rc = check_blocks("mofo_diff_attention_fwd", std::max(grid_of(a, pl.nx * pl.nsplit), grid_of(a, pl.tail)));
+    if (rc) return rc;
+    const dim3 grid((unsigned)grid_of(a, pl.nx * pl.nsplit));
     hipStream_t s = (hipStream_t)stream;
     auto four_way_rows = [&](int nx) {
-        const dim3 g(grid_of(a, nx));
+        const dim3 g((unsigned)grid_of(a, nx));
         if (o) hipLaunchKernelGGL((diff_fwd_kernel<true, true, false>), g, dim3(256), 0, s, a, f, nx, 1, spread);
         else hipLaunchKernelGGL((diff_fwd_kernel<true, false, false>), g, dim3(256), 0, s, a, f, nx, 1, spread);
     };
@@ -1563,8 +1570,6 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     float* part = ws + rows * 4 + (gamma ? rows * (HV / 2) : 0);
     float* lams = part + (size_t)H * row_blocks(B, Nq, H) * (HV + 1);
     const int nb = row_blocks(B, Nq, H);
-    hipLaunchKernelGGL(diff_rows_kernel, dim3(nb, H), dim3(256), 0, s, a, (const bf16_t*)o, (const bf16_t*)o2, (const bf16_t*)dout, (size_t)lddo, lse2, d_o, stats, part, lams);
-    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
     const bf16_t* dy = gamma ? d_o : (const bf16_t*)dout;
     const size_t lddy = gamma ? (size_t)H * HV : (size_t)lddo;
     const long long groups = (long long)B * Hkv, kt = (Nk + 31) / 32, qt = (long long)a.G * ((Nq + 31) / 32);
@@ -1585,21 +1590,27 @@ extern "C" int mofo_diff_attention_bwd(const void* q, int ldq, const void* k, in
     g.params = lam_heads + (dgamma ? 16 : 0);
     g.np = (g.params + 7) / 8 * 8;
     g.nxk = ceil_div(Nk, k4 ? 32 : 128);
-    g.nk = (int)grid_of(a, g.nxk);
+    const long long nk_blocks = grid_of(a, g.nxk);
     g.nxq = q4 ? ceil_div(a.R, 32) : (int)cut.nx;
     g.spread = spread_of(a);
-    const dim3 grid(g.np + g.nk + grid_of(a, g.nxq));
+    const int tail = q4 ? 0 : tail_blocks(cut, a.R);
+    const long long blocks = g.np + nk_blocks + grid_of(a, g.nxq);
+    rc = check_blocks("mofo_diff_attention_bwd", std::max(blocks, grid_of(a, tail)));
+    if (rc) return rc;
+    g.nk = (int)nk_blocks;
+    hipLaunchKernelGGL(diff_rows_kernel, dim3(nb, H), dim3(256), 0, s, a, (const bf16_t*)o, (const bf16_t*)o2, (const bf16_t*)dout, (size_t)lddo, lse2, d_o, stats, part, lams);
+    MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(rows)");
+    const dim3 grid((unsigned)blocks);
     if (q4 && k4) hipLaunchKernelGGL((diff_grad_kernel<true, true>), grid, dim3(256), 0, s, g);
     else if (q4) hipLaunchKernelGGL((diff_grad_kernel<true, false>), grid, dim3(256), 0, s, g);
     else if (k4) hipLaunchKernelGGL((diff_grad_kernel<false, true>), grid, dim3(256), 0, s, g);
     else hipLaunchKernelGGL((diff_grad_kernel<false, false>), grid, dim3(256), 0, s, g);
     MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(gradients)");
-    const int tail = q4 ? 0 : tail_blocks(cut, a.R);
     if (tail) {
         g.a.row0 = g.nxq * 128;
         g.np = g.params = g.nk = 0;
         g.nxq = tail;
-        hipLaunchKernelGGL((diff_grad_kernel<true, false>), dim3(grid_of(a, tail)), dim3(256), 0, s, g);
+        hipLaunchKernelGGL((diff_grad_kernel<true, false>), dim3((unsigned)grid_of(a, tail)), dim3(256), 0, s, g);
         MOFO_CHECK_LAUNCH("mofo_diff_attention_bwd(last rows)");
     }
     return MOFO_OK;

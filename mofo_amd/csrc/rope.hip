@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeArgs a) {
 
 template <bool BF, bool INTER>
 void launch(const RopeArgs& a, int inverse, hipStream_t s) {
-    const dim3 grid((unsigned)ceil_div(a.M, a.tok_per_block));
+    const dim3 grid((unsigned)(((long long)a.M + a.tok_per_block - 1) / a.tok_per_block));
     if (inverse) hipLaunchKernelGGL((rope_axes_kernel<BF, INTER, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((rope_axes_kernel<BF, INTER, false>), grid, dim3(256), 0, s, a);
 }
@@ -151,6 +151,13 @@ extern "C" int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, 
                                {"pos", pos, 1, (long long)M * naxes * 4, 0}, {"tok_idx", tok_idx, 1, (long long)M * 4, 0}};
         MOFO_CHECK_APART("mofo_rope_axes", &o, 1, in, 4);
     }
+    // few tokens: one a block, to fill the card (160 tokens x 24 heads in bf16, us by tokens a block: 1 3.1, 4 3.7, 8 4.2; 2048 4.5, 4.6, 5.0);
+    // many: several, for the angles' share of a block's time (8192 12.4, 9.7, 9.8; 50176 76, 57, 58), more of them if their rows are short
+    // (50176 x 3 heads 39, 15, 13; 14997 x 7 heads in f32: 4 11.7, 8 11.2)
+    const int tok_per_block = M < 2048 ? 1 : W * (x_is_bf16 ? 2 : 4) >= 2048 ? ROPE_TOK / 2 : ROPE_TOK;
+    const long long blocks = ((long long)M + tok_per_block - 1) / tok_per_block;
+    if (blocks > MOFO_MAX_BLOCKS_256)
+        MOFO_FAIL(MOFO_EUNSUPPORTED, "mofo_rope_axes: M=%d takes %lld blocks of %d rows (at most %lld)", M, blocks, tok_per_block, MOFO_MAX_BLOCKS_256);
     RopeArgs a;
     a.x = x;
     a.out = out;
@@ -170,10 +177,7 @@ extern "C" int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, 
     a.gh = grid_h;
     a.gw = grid_w;
     a.in_place = x == out;
-    // few tokens: one a block, to fill the card (160 tokens x 24 heads in bf16, us by tokens a block: 1 3.1, 4 3.7, 8 4.2; 2048 4.5, 4.6, 5.0);
-    // many: several, for the angles' share of a block's time (8192 12.4, 9.7, 9.8; 50176 76, 57, 58), more of them if their rows are short
-    // (50176 x 3 heads 39, 15, 13; 14997 x 7 heads in f32: 4 11.7, 8 11.2)
-    a.tok_per_block = M < 2048 ? 1 : W * (x_is_bf16 ? 2 : 4) >= 2048 ? ROPE_TOK / 2 : ROPE_TOK;
+    a.tok_per_block = tok_per_block;
     hipStream_t s = (hipStream_t)stream;
     if (x_is_bf16) {
         if (interleaved) launch<true, true>(a, inverse, s);

@@ -96,3 +96,34 @@ def test_rope_frequencies():
     want = [1.0, 100.0 ** -0.5, 1.0, 100.0 ** (-1 / 3), 100.0 ** (-2 / 3), 1.0]
     assert f.dtype == torch.float64 and torch.allclose(f * 2 * math.pi, torch.tensor(want, dtype=torch.float64), rtol=1e-15, atol=0)
     assert ops.rope_freqs((0, 8, 0), device="cpu").numel() == 8
+
+
+BIG = 1 << 36   # as P, for tensors of many GiB
+
+
+@pytest.mark.parametrize("bad", [
+    dict(M=1 << 27, heads=1, hd=16, ldx=16, ldo=16, naxes=1, sections=(8, 0, 0, 0)), dict(M=(1 << 27) + 1, heads=2, hd=64, bf=0),
+    dict(M=1 << 26, heads=16, hd=64, ldx=1024, ldo=1024), dict(M=1 << 30, heads=1, hd=64, ldx=64, ldo=64)])
+def test_rope_entry_refuses_more_blocks_than_a_launch_takes(bad):
+    """2^24 blocks of 256 threads are 2^32 threads, one more than a launch counts"""
+    a = dict(x=BIG, out=8 * BIG, freqs=P, pos=16 * BIG)
+    assert _rope(**{**a, **bad}) < 0 and "blocks" in _error()
+
+
+MANY = [dict(B=1 << 20, Nq=1, Nk=1, H=16, Hkv=16), dict(B=1 << 24, Nq=1, Nk=1, H=1, Hkv=1), dict(B=1 << 22, Nq=1, Nk=1, H=8, Hkv=4), dict(B=1 << 20, Nq=17, Nk=17, H=16, Hkv=16)]
+
+
+@pytest.mark.parametrize("bad", MANY)
+def test_diff_attention_entry_refuses_more_blocks_than_a_launch_takes(bad):
+    w = bad["H"] * 128
+    a = dict(q=BIG, ldq=w, k=4 * BIG, ldk=w, v=8 * BIG, ldv=w, out=12 * BIG, ldo=w, lam_heads=1)
+    assert _fwd(**{**a, **bad}) < 0 and "mofo_diff_attention_fwd" in _error() and "blocks" in _error()
+
+
+@pytest.mark.parametrize("bad", MANY + [dict(B=1 << 19, Nq=1, Nk=1, H=16, Hkv=16)])
+def test_diff_attention_gradient_entry_refuses_more_blocks_than_a_launch_takes(bad):
+    """dK / dV, dQ and the parameters' blocks are one launch: half as many (clip, key head) pairs fill it"""
+    w = bad["H"] * 128
+    a = dict(q=BIG, ldq=w, k=4 * BIG, ldk=w, v=8 * BIG, ldv=w, lam_heads=1, o=12 * BIG, o2=16 * BIG, lse2=20 * BIG, dout=24 * BIG, lddo=w, dq=28 * BIG, lddq=w,
+             dk=32 * BIG, lddk=w, dv=36 * BIG, lddv=w, ws=40 * BIG, n=1 << 40)
+    assert _bwd(**{**a, **bad}) < 0 and "mofo_diff_attention_bwd" in _error() and "blocks" in _error()
