@@ -531,7 +531,10 @@ def _pitch(dev, dtype, name, t):
     if t is not None:
         s = t.stride()
         if len(s) == 2 and s[1] == 1 and t.dtype is dtype and t.get_device() == dev:
-            return s[0] if t.shape[0] > 1 else t.shape[1]
+            ld = s[0] if t.shape[0] > 1 else t.shape[1]
+            if ld >> 31:                                    # the entries' ints: the low 32 bits would be another pitch
+                raise ValueError(f"{name}: a row pitch of {ld} elements (below 2^31)")
+            return ld
     _chk(t, dtype, name, 2)
     raise ValueError(f"{name} must be on the current device cuda:{dev}, it is on {t.device}")
 
@@ -563,6 +566,8 @@ def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, int
     _dev_chk(dev, torch.float64, 1, freqs=freqs)
     shape, axes = x.shape, len(sections)
     M = shape[0]
+    if M >> 31:
+        raise ValueError(f"rope_axes: {M} rows (below 2^31)")
     pairs, sections = _rope_sections(tuple(sections), head_dim)
     if shape[1] != heads * head_dim or out.shape != shape:
         raise ValueError(f"rope_axes: {nx} and {nout} must be [M, heads * head_dim]")
@@ -580,6 +585,8 @@ def _rope_axes(x, heads, head_dim, sections, freqs, out, pos, tok_idx, grid, int
         if tok_idx.numel() != M or not tok_idx.is_contiguous() or axes != 3 or grid is None or len(grid) != 3:
             raise ValueError("rope_axes: tok_idx must hold M contiguous ids, with three sections and a grid (T, H, W)")
         gh, gw = grid[1], grid[2]
+        if gh >> 31 or gw >> 31:
+            raise ValueError(f"rope_axes: a grid of {gh} x {gw} places")
     if M:
         _run("mofo_rope_axes", ("rope",), 2.0 * x.numel() * x.element_size(), x.data_ptr(), 1 if dt is BF16 else 0, ldx, out.data_ptr(), ldo, M,
              heads, head_dim, freqs.data_ptr(), axes, sections, _p(pos), _p(tok_idx), gh, gw, 1 if interleaved else 0, 1 if inverse else 0)

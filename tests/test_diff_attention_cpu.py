@@ -127,3 +127,15 @@ def test_diff_attention_gradient_entry_refuses_more_blocks_than_a_launch_takes(b
     a = dict(q=BIG, ldq=w, k=4 * BIG, ldk=w, v=8 * BIG, ldv=w, lam_heads=1, o=12 * BIG, o2=16 * BIG, lse2=20 * BIG, dout=24 * BIG, lddo=w, dq=28 * BIG, lddq=w,
              dk=32 * BIG, lddk=w, dv=36 * BIG, lddv=w, ws=40 * BIG, n=1 << 40)
     assert _bwd(**{**a, **bad}) < 0 and "mofo_diff_attention_bwd" in _error() and "blocks" in _error()
+
+
+def test_wrappers_refuse_pitches_that_do_not_fit_the_entries():
+    """the C entries take row pitches as 32-bit ints: a pitch of 2^32 + 512 elements is not one of 512"""
+    from mofo_amd import ops
+    for pitch, ok in ((512, True), ((1 << 31) - 8, True), (1 << 31, False), ((1 << 32) + 512, False)):
+        t = torch.empty_strided((2, 128), (pitch, 1), dtype=torch.bfloat16, device="meta")
+        if ok:
+            assert ops._pitch(-1, torch.bfloat16, "q", t) == pitch
+        else:
+            with pytest.raises(ValueError, match="pitch"):
+                ops._pitch(-1, torch.bfloat16, "q", t)

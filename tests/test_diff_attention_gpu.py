@@ -684,3 +684,26 @@ def test_diff_attention_gradients_of_rows_that_see_nothing_are_not_taken(dev, no
         got = _call(*args(q2), dout=d2)
         for n in want:
             assert torch.equal(got[n], want[n]), (n, bad)
+
+
+def test_row_pitches_and_counts_that_do_not_fit_the_entries_are_refused(dev):
+    """two rows 2^32 + 512 elements apart (a pitch whose low 32 bits would do), a grid and a number of rows beyond 32 bits"""
+    from mofo_amd import ops
+    big = torch.zeros((1 << 32) + 1024, dtype=BF16, device=dev)
+    far = lambda n: big.as_strided((2, n), ((1 << 32) + 512, 1))  # noqa: E731
+    x, lam = _rand((2, 128), dev, 1), _rand((4, 1, 64), dev, 2, 0.1)
+    f, pos, tok = ops.rope_freqs((8, 12, 12), device=dev), torch.zeros(2, 3, dtype=I32, device=dev), torch.zeros(2, dtype=I32, device=dev)
+    out, ws = torch.empty_like(x), torch.empty(1 << 16, dtype=F32, device=dev)
+    saved = (torch.empty_like(x), torch.empty_like(x), torch.empty(2, 1, 1, 2, dtype=F32, device=dev))
+    attend = lambda **kw: ops.diff_attention_fwd(**{**dict(q=x, k=x, v=x, B=1, H=1, Hkv=1, scale=0.125, lam=lam, lam_init=0.4, out=out), **kw})  # noqa: E731
+    back = lambda **kw: ops.diff_attention_bwd(**{**dict(q=x, k=x, v=x, B=1, H=1, Hkv=1, scale=0.125, lam=lam, lam_init=0.4, saved=saved, dout=x, dq=torch.empty_like(x),  # noqa: E731
+                                                         dk=torch.empty_like(x), dv=torch.empty_like(x), dlam=torch.empty_like(lam), ws=ws), **kw})
+    for bad in (lambda: ops.rope_axes_fwd(far(128), 2, 64, (8, 12, 12), f, out, pos=pos), lambda: ops.rope_axes_bwd(x, 2, 64, (8, 12, 12), f, far(128), pos=pos),
+                lambda: attend(q=far(128)), lambda: attend(k=far(128)), lambda: attend(v=far(128)), lambda: attend(out=far(128)), lambda: back(dout=far(128)),
+                lambda: back(dq=far(128)), lambda: back(dk=far(128)), lambda: back(dv=far(128)),
+                lambda: ops.rope_axes_fwd(x, 2, 64, (8, 12, 12), f, out, tok_idx=tok, grid=(8, (1 << 32) + 14, 14))):
+        with pytest.raises(ValueError):
+            bad()
+    rows = torch.zeros(16, dtype=BF16, device=dev).expand((1 << 32) + 1, 16)
+    with pytest.raises(ValueError, match="rows"):
+        ops.rope_axes_fwd(rows, 1, 16, (8,), ops.rope_freqs((8,), device=dev), rows, tok_idx=tok, grid=(8, 14, 14))
