@@ -29,6 +29,10 @@ constexpr float EMPTY_LSE = 1.0e30f;    // log-sum of a row that sees nothing: e
 // far above it, which is then 1 and not rounded at all.  (Gradients are formed from differences G - d in which such a term cancels: with
 // the sum of the unrounded terms and a reference kept up to 2^20, dq of 160 and 50 tokens was 6e-3 and 1e-2 off; this way 3e-3.)
 constexpr float KEEP_REF = 5.f;
+// Exponents are c s - c (reference) in one fused step while the references of a wave's rows lie below this many log2 units: the rounding of
+// c (reference), 2^-15, is the same for all of a row's terms of one reference, and that small against those of another.  Once one lies
+// beyond, the wave forms the differences first, exactly, at one more instruction a term, and takes every tile's maximum for reference.
+constexpr float FAR_REF = 1024.f;
 
 struct DiffArgs {
     const bf16_t *q, *k, *v;
@@ -296,7 +300,7 @@ struct FwdOut {
     size_t ldo;
     float* lse2;              // [2][B][H][Nq] or NULL
     float* part;              // nsplit > 1: [rows][nsplit][2][128] outputs of a range of keys, divided by its own sum, then
-    float* part_lse;          // [rows][nsplit][2] its log2-sum (-inf: nothing seen); rows = B * H * Nq
+    f32x2* part_stat;         // [rows][nsplit][2] its reference (score units) and its log2-sum against it (both -inf: nothing seen); rows = B * H * Nq
 };
 
 // sum of the eight rounded terms of a fragment
@@ -392,7 +396,8 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
     }
 
     const FragOff fo = frag_off(lds0 + ring, lane);
-    const float keep = KEEP_REF / a.c;                    // in score units
+    float keep = KEEP_REF / a.c;                          // in score units; far references: -inf, every tile takes the branch below
+    float cm = a.c;                                       // what the reference is scaled with in an exponent: 0 where the difference is formed first
     for (int t = 0; t < nkt; ++t) {
         if constexpr (KEYS4) {
             landed_own();
@@ -435,12 +440,13 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
             tm[m] = s[m][0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) tm[m] = fmaxf(tm[m], s[m][r]);
+            if (m == 0) __builtin_amdgcn_sched_barrier(0);      // the first map's maximum while the second's scores are on their way
         }
         if (__any(tm[0] > mx[0] + keep || tm[1] > mx[1] + keep)) {            // the first tile (reference -inf) too
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 const float x = fmaxf(tm[m], __shfl_xor(tm[m], 32, 64));
-                const bool up = x > mx[m] + keep;
+                const bool up = x > mx[m] + (cm == 0.f ? 0.f : keep);
                 const float alpha = up ? fast_exp2((mx[m] - x) * a.c) : 1.f;
                 mx[m] = up ? x : mx[m];
                 l[m] *= alpha;
@@ -450,9 +456,18 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
             }
+            auto is_far = [&](float x) { return x > -__builtin_inff() && fabsf(x * a.c) > FAR_REF; };
+            if (cm == 0.f || __ballot(is_far(mx[0]) || is_far(mx[1])) != 0) {
+                cm = 0.f;
+                keep = -__builtin_inff();
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[m][r] -= mx[m];
+            }
         }
         // two halves of 16 keys: the second half's exponentials stand beside the first half's products
-        const float nmc[2] = {-mx[0] * a.c, -mx[1] * a.c};
+        const float nmc[2] = {-mx[0] * cm, -mx[1] * cm};
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             if (KEYS4 && s2 == 1) {
@@ -487,7 +502,16 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
         lt[m] = l[m] + __shfl_xor(l[m], 32, 64);
         lx[m] = SAVE ? le[m] + __shfl_xor(le[m], 32, 64) : lt[m];
     }
-    float inv[2], lse[2];
+    float inv[2];
+    // a row's statistics leave as soon as they are known: the map's reference (score units) and the sum of its terms against that
+    int row_lane = lane & 31;
+    asm volatile("" : "+v"(row_lane));                    // the row's place is made anew: kept through the loop it would not fit the registers
+    const Row at = make_row(a, kvh, r0 + row_lane, len);
+    auto put_stat = [&](int m, bool seen, float ref, float sum) {
+        if (!at.valid || hh != 0 || (KEYS4 && wave != 0)) return;
+        if constexpr (SPLIT) f.part_stat[(stat_at(a, b, at) * nsplit + sp) * 2 + m] = seen ? f32x2{ref, fast_log2(sum)} : f32x2{-__builtin_inff(), -__builtin_inff()};
+        else if constexpr (SAVE) f.lse2[(size_t)m * a.B * a.H * a.Nq + stat_at(a, b, at)] = seen ? ref * a.c + fast_log2(sum) : EMPTY_LSE;
+    };
     float* xch = (float*)(smem + XCH);
     if constexpr (KEYS4) {
         // the four waves' references and sums, [wave][map][reference, rounded sum, sum][32 rows]; a wave without keys of the row: nothing
@@ -519,7 +543,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
                 sx += e * p[64];
             }
             inv[m] = some ? fast_exp2((mx[m] - top) * a.c) / st : 0.f;
-            lse[m] = top * a.c + fast_log2(sx);
+            put_stat(m, any, top, sx);
         }
         // a map at a time (there is no room for both); wave w goes on with columns 32 w .. 32 w + 31
         f32x16 sum[2];
@@ -547,19 +571,14 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             inv[m] = some ? 1.0f / lt[m] : 0.f;
-            lse[m] = mx[m] * a.c + fast_log2(lx[m]);
+            put_stat(m, some, mx[m], lx[m]);
         }
     }
     constexpr int ND = KEYS4 ? 1 : 4;                     // column tiles this wave still holds, from dt0 on
     const int dt0 = KEYS4 ? wave : 0;
     if constexpr (SPLIT) {
-        if (!w.valid) return;
-        const size_t pi = stat_at(a, b, w) * nsplit + sp;
-        if (all <= 0) {                                   // the join does not read a range of weight zero
-            if (hh == 0 && (!KEYS4 || wave == 0)) f.part_lse[pi * 2] = f.part_lse[pi * 2 + 1] = -__builtin_inff();
-            return;
-        }
-        float* pp = f.part + pi * (2 * HV);
+        if (!at.valid || all <= 0) return;                // the join does not use a range of weight zero
+        float* pp = f.part + (stat_at(a, b, at) * nsplit + sp) * (2 * HV);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -571,7 +590,6 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
                     for (int e = 0; e < 4; ++e) x[e] = some ? o[m][dt][4 * rg + e] * inv[m] : 0.f;
                     *(f32x4*)(pp + m * HV + 32 * (dt0 + dt) + 8 * rg + 4 * hh) = x;
                 }
-            if (hh == 0 && (!KEYS4 || wave == 0)) f.part_lse[pi * 2 + m] = some ? lse[m] : -__builtin_inff();
         }
     } else {
     __syncthreads();                                      // the ring is free, the sums are read
@@ -601,10 +619,6 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) out_put16(lds + NEXT, lane, dt0 + dt, o[0][dt], 1.f);
         if (!KEYS4) out_flush(lds, lane, [&](int r) { return list_row(a, f.o, HW, b, kvh, r0 + r); });
-        if (w.valid && hh == 0 && (!KEYS4 || wave == 0)) {
-#pragma unroll
-            for (int m = 0; m < 2; ++m) f.lse2[(size_t)m * a.B * a.H * a.Nq + stat_at(a, b, w)] = some ? lse[m] : EMPTY_LSE;
-        }
     }
     if (a.gamma) {
         ss += __shfl_xor(ss, 32, 64);
@@ -642,15 +656,16 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 }
 
 // joins the ranges of a row: one wave a row, lanes 0..31 the first map's 128 columns, lanes 32..63 the second's; the ranges' weights are
-// exp2(lse_range - lse), lane s of a half holding ranges s and s + 32.  A chain of latencies: the first sixteen ranges' loads go out before
-// anything is waited for (one token against 16 caches of 8192, 16 ranges: 5.5 us, 6.5 in rounds of eight behind the weights).
+// exp2(c (reference - largest reference) + log2-sum) over their sum, lane s of a half holding ranges s and s + 32.  A chain of latencies: the
+// first sixteen ranges' loads go out before anything is waited for (one token against 16 caches of 8192, 16 ranges: 5.5 us, 6.5 in rounds of eight behind the weights).
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, int nsplit) {
     constexpr int AT_ONCE = 16;
     const int lane = threadIdx.x & 63, m = lane >> 5, sl = lane & 31, d = sl * 4;
     const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (size_t)a.B * a.H * a.Nq;
     if (row >= rows) return;
-    const float* pl = f.part_lse + row * nsplit * 2 + m;
-    const float v0 = sl < nsplit ? pl[2 * sl] : -__builtin_inff(), v1 = sl + 32 < nsplit ? pl[2 * (sl + 32)] : -__builtin_inff();
+    const f32x2* pl = f.part_stat + row * nsplit * 2 + m;
+    const f32x2 nothing = {-__builtin_inff(), -__builtin_inff()};
+    const f32x2 v0 = sl < nsplit ? pl[2 * sl] : nothing, v1 = sl + 32 < nsplit ? pl[2 * (sl + 32)] : nothing;
     const float* pp = f.part + row * nsplit * (2 * HV) + m * HV + d;
     f32x4 x[AT_ONCE];
     auto fetch = [&](int s0) {
@@ -667,14 +682,15 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, in
     }
     float e1, e2;
     const float lam = head_lambda(a, h, lane, e1, e2);
-    float top = fmaxf(v0 != v0 ? __builtin_inff() : v0, v1 != v1 ? __builtin_inff() : v1);        // a NaN of any range makes the row NaN
+    float top = fmaxf(v0[0], v1[0]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const bool none = top == -__builtin_inff();
-    float w0 = none ? 0.f : fast_exp2(v0 - top), w1 = none ? 0.f : fast_exp2(v1 - top), sum = w0 + w1;
+    // a NaN among a range's scores leaves its log-sum NaN, and makes the row NaN
+    const bool none = (uint32_t)(__ballot(v0[1] != -__builtin_inff() || v1[1] != -__builtin_inff()) >> (lane & 32)) == 0;
+    float w0 = none ? 0.f : fast_exp2(fmaf(v0[0] - top, a.c, v0[1])), w1 = none ? 0.f : fast_exp2(fmaf(v1[0] - top, a.c, v1[1])), sum = w0 + w1;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float lse = none ? EMPTY_LSE : top + fast_log2(sum), inv = none ? 0.f : 1.0f / sum;
+    const float lse = none ? EMPTY_LSE : top * a.c + fast_log2(sum), inv = none ? 0.f : 1.0f / sum;
     w0 *= inv;
     w1 *= inv;
     f32x4 acc = {0, 0, 0, 0};
@@ -1382,7 +1398,7 @@ DiffArgs make_args(const void* q, int ldq, const void* k, int ldk, const void* v
     return a;
 }
 
-constexpr int PART = 2 * HV + 2;        // floats of workspace per row and range
+constexpr int PART = 2 * HV + 4;        // floats of workspace per row and range
 
 // Which block form, from a model of the time on 256 compute units that its measurements gave, us:
 //   128 rows (keys) a block, `steps` 32 x 32 tiles in a row    6.8 + 0.92 steps, two blocks on a compute unit 1.45 times that
@@ -1490,7 +1506,7 @@ extern "C" int mofo_diff_attention_fwd(const void* q, int ldq, const void* k, in
     FwdOut f = {(bf16_t*)out, (bf16_t*)o, (bf16_t*)o2, (size_t)ldo, lse2, nullptr, nullptr};
     if (pl.nsplit > 1) {
         f.part = ws;
-        f.part_lse = ws + rows * pl.nsplit * (2 * HV);
+        f.part_stat = (f32x2*)(ws + rows * pl.nsplit * (2 * HV));
     }
     const int spread = spread_of(a);
     rc = check_blocks("mofo_diff_attention_fwd", std::max(grid_of(a, pl.nx * pl.nsplit), grid_of(a, pl.tail)));

@@ -707,3 +707,58 @@ def test_row_pitches_and_counts_that_do_not_fit_the_entries_are_refused(dev):
     rows = torch.zeros(16, dtype=BF16, device=dev).expand((1 << 32) + 1, 16)
     with pytest.raises(ValueError, match="rows"):
         ops.rope_axes_fwd(rows, 1, 16, (8,), ops.rope_freqs((8,), device=dev), rows, tok_idx=tok, grid=(8, 14, 14))
+
+
+def _far_scores(dev, B, Nq, Nk, H, Hkv, offset, seed=0):
+    """whole-numbered inputs whose scores are ``offset`` + small whole numbers, exact in 32 bits in any order of the sums (all below 2^24 in size);
+    the offset's sign is the query row's and the map's own"""
+    g = torch.Generator().manual_seed(seed)
+    whole = lambda *s: torch.randint(-2, 3, s, generator=g).to(F32)  # noqa: E731
+    a = 2.0 ** (math.frexp(offset)[1] // 2)
+    q, k, v = whole(B * Nq, H, 2, 64), whole(B * Nk, Hkv, 2, 64), torch.randn(B * Nk, Hkv * 128, generator=g)
+    sign = torch.randint(0, 2, (B * Nq, H, 2), generator=g) * 2.0 - 1
+    q[..., 0], k[..., 0] = sign * a, offset / a
+    lam = (torch.randn(4, H, 64, generator=g) * 0.1).to(F32).to(dev)
+    return q.reshape(B * Nq, -1).to(BF16).to(dev), k.reshape(B * Nk, -1).to(BF16).to(dev), v.to(BF16).to(dev), lam
+
+
+FAR = [  # B, Nq, Nk, H, Hkv, causal: ranges of keys, four-way blocks, 128-row blocks, 128-row blocks with a causal mask
+    (2, 1, 4000, 4, 2, 2), (1, 3, 2500, 2, 2, 0), (1, 300, 300, 2, 1, 1), (24, 140, 140, 12, 12, 0), (67, 100, 100, 8, 4, 1)]
+
+
+@pytest.mark.parametrize("offset", [2.0 ** 12, 2.0 ** 16, 2.0 ** 22])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_scores_far_from_zero(dev, B, Nq, Nk, H, Hkv, causal, offset):
+    """soft maps whose scores all lie far from zero: exponents are differences, so the size of the scores costs the outputs nothing.  (The scores
+    themselves are exact here; lse2 is one 32-bit number of the scores' size.)  With and without what the gradient wants."""
+    q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, offset)
+    args = (q, k, v, B, H, Hkv, 0.125, lam, 0.45, None, 1.0, None, causal)
+    want = _reference(*args)
+    _check(_call(*args), want, 0.01)
+    from mofo_amd import ops
+    saved = (torch.empty_like(q), torch.empty_like(q), torch.empty(2, B, H, Nq, dtype=F32, device=dev))
+    out, ws = torch.empty_like(q), torch.empty(ops.diff_attention_fwd_ws(B, Nq, Nk, H, Hkv), dtype=F32, device=dev)
+    ops.diff_attention_fwd(q, k, v, B, H, Hkv, 0.125, lam, 0.45, out, saved=saved, ws=ws, causal=causal)
+    _check(dict(out=out, o=saved[0], o2=saved[1], lse2=saved[2]), want, 0.01)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_scores_of_any_size(dev, B, Nq, Nk, H, Hkv, causal):
+    """every score the same number, 1.4 * 2^106 (times the scale), of either sign: the maps are uniform"""
+    q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, 181 * 2.0 ** 99)
+    q.view(-1, 64)[:, 1:] = 0
+    args = (q, k, v, B, H, Hkv, 0.125, lam, 0.45, None, 1.0, None, causal)
+    _check(_call(*args), _reference(*args), 0.01)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_scores_that_come_near(dev, B, Nq, Nk, H, Hkv, causal):
+    """the keys' scores lie 2^16 (times the scale) from zero at the start and near it from a third of the keys on: on either side of it by the row,
+    and below it in every row, so that no row's reference stays far"""
+    q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, 2.0 ** 16)
+    k.view(B, Nk, -1, 64)[:, Nk // 3:, :, 0] = 1.0 / 256
+    for below in (False, True):
+        if below:
+            q.view(-1, 64)[:, 0] = -q.view(-1, 64)[:, 0].abs()
+        args = (q, k, v, B, H, Hkv, 0.125, lam, 0.45, None, 1.0, None, causal)
+        _check(_call(*args), _reference(*args), 0.01)
