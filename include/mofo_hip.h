@@ -209,6 +209,9 @@ int mofo_rope_axes(const void* x, int x_is_bf16, int ldx, void* out, int ldo, in
  * the gradients.  Rows of k, v at and behind kv_len[b] may hold anything; rows in front of it are expected to be finite.
  * scale: 2^-24 .. 2^24; eps (with gamma): at least 2^-100.  A launch takes at most 2^24 - 1 blocks (a (clip, key head) pair's lists of 32 or 128
  * rows, and in the gradient of keys too); calls of more are refused before anything is launched.
+ * The outputs are right at any size of the scores (scale q.k, formed in 32 bits); the gradient forms P again from lse2, one 32-bit number
+ * a row and map, which leaves it up to |score| * 2^-21 of its value off: 2^-9, half a rounding to bf16, at |score| = 2^12.  Scores
+ * beyond that are not for training.
  * For the gradient keep o, o2 (bf16 [B * Nq, H * 128], contiguous) and lse2 (f32 [2, B, H, Nq], log2-sum-exp2); NULL all three otherwise.
  * ws: mofo_diff_attention_fwd_ws floats of scratch (0: NULL is fine), contents of no interest; two calls that may run at once (two
  * streams, two captured graphs) need one each. ---- */

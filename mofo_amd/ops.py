@@ -692,7 +692,8 @@ def diff_attention_fwd(q, k, v, B, H, Hkv, scale, lam, lam_init, out, gamma=None
 def diff_attention_bwd(q, k, v, B, H, Hkv, scale, lam, lam_init, saved, dout, dq, dk, dv, dlam, ws, gamma=None, dgamma=None, eps=1e-5, out_scale=1.0,
                        kv_len=None, causal=0):
     """every gradient of ``diff_attention_fwd`` (same arguments, its ``saved``), overwritten: ``dq``, ``dk``, ``dv`` bf16 like q, k, v, ``dlam`` (and
-    ``dgamma``) f32 or bf16 like lam (gamma).  ``ws``: f32, diff_attention_bwd_ws elements."""
+    ``dgamma``) f32 or bf16 like lam (gamma).  ``ws``: f32, diff_attention_bwd_ws elements.  For scores (scale * q.k) of up to 2^12: the
+    probabilities are formed again from 32-bit log-sums and are up to |score| * 2^-21 of their value off."""
     who = "diff_attention_bwd"
     dev, Nq, Nk, (ldq, ldk, ldv) = _diff_chk(who, q, k, v, B, H, Hkv, lam, gamma, kv_len, causal, ws)
     o, o2, lse2 = _diff_saved(who, dev, saved, B, Nq, H)

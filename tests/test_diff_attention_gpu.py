@@ -762,3 +762,32 @@ def test_diff_attention_scores_that_come_near(dev, B, Nq, Nk, H, Hkv, causal):
             q.view(-1, 64)[:, 0] = -q.view(-1, 64)[:, 0].abs()
         args = (q, k, v, B, H, Hkv, 0.125, lam, 0.45, None, 1.0, None, causal)
         _check(_call(*args), _reference(*args), 0.01)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_gradients_of_scores_far_from_zero(dev, B, Nq, Nk, H, Hkv, causal):
+    """scores about +-2^12, the size up to which the gradient's probabilities are promised to 2^-9 of their value: that in the place of F,
+    2^-14, is 32 times F.  2-norms: the usual 2 %, and twice 2^-9 for the difference of two maps; without the columns of the offset, where dq
+    and dk are sums that cancel to nothing."""
+    q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, 2.0 ** 15)
+    dout = _rand((B * Nq, H * 128), dev, 5)
+    args = (q, k, v, B, H, Hkv, 0.125, lam, 0.45, None, 1.0, None, causal)
+    got, want = _call(*args, dout=dout, grads=F32), _reference(*args, dout=dout, grad_u=0.0)
+    _check(got, {n: (t, b * (32.0 if n.startswith("d") else 1.0)) for n, (t, b) in want.items()})
+    for n in ("dq", "dk", "dv"):
+        a, b = (t.double().reshape(t.shape[0], -1, 64)[..., 1 if n != "dv" else 0:] for t in (got[n], want[n][0]))
+        assert _rel(a, b) < 0.02 + 2 * 2.0 ** -9, (n, _rel(a, b))
+
+
+@pytest.mark.parametrize("power", [-21, 27])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_same_bits_at_any_scale(dev, B, Nq, Nk, H, Hkv, causal, power):
+    """the ends of the scale, 2^-24 and 2^24, with the same scores: powers of two move from q and k into the scale, and back out of dq and dk"""
+    q, k, v, lam, gamma, dout = _case(dev, B, Nq, Nk, H, Hkv, True)
+    half, rest = 2.0 ** -(power // 2), 2.0 ** -(power - power // 2)
+    form = (lam, 0.45, gamma, 0.55, None, causal)
+    want = _call(q, k, v, B, H, Hkv, 0.125, *form, dout=dout)
+    got = _call(q * half, k * rest, v, B, H, Hkv, 0.125 * 2.0 ** power, *form, dout=dout)
+    for n in want:
+        scaled = {"dq": 1 / half, "dk": 1 / rest}.get(n, 1.0)
+        assert torch.equal(got[n], want[n] * scaled), n
