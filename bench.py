@@ -533,20 +533,16 @@ def main():
         # (tools/pmc_step.sh; FETCH_SIZE doubled as the guide prescribes for gfx950).  Counters cannot be read from inside the
         # process, so this is a RECORDED figure: it is reported only while the kernel sources are byte-identical to the ones
         # the profile was taken with (sha256 over mofo_amd/csrc), null otherwise.
-        import glob
-        recs = sorted(glob.glob(os.path.join(ROOT, "profiles", "r*_pmc_step_traffic.json")))
-        tpath = recs[-1] if recs else ""               # the newest round's record
-        tname = "profiles/" + os.path.basename(tpath)
         out["roofline"]["traffic_source"] = None
-        if args.model == "vitb16" and B == 32 and os.path.exists(tpath):   # recorded for the headline workload only
+        if args.model == "vitb16" and B == 32:         # recorded for the headline workload only
             try:
-                prof_rec = json.load(open(tpath))
-                rec = prof_rec.get("classes", {}).get(out["roofline"]["kernel"])
-                if prof_rec.get("_meta", {}).get("csrc_sha256") != csrc_sha():
-                    out["roofline"]["traffic_source"] = "stale: %s was recorded for other kernel sources" % tname
+                tname, prof_rec = traffic_record(os.path.join(ROOT, "profiles"), csrc_sha())
+                rec = prof_rec.get("classes", {}).get(out["roofline"]["kernel"]) if prof_rec else None
+                if tname and prof_rec is None:
+                    out["roofline"]["traffic_source"] = "stale: profiles/%s was recorded for other kernel sources" % tname
                 elif rec:
                     out["roofline"]["traffic"] = round((rec["fetch_MB_per_launch"] + rec["write_MB_per_launch"]) * 1e6)
-                    out["roofline"]["traffic_source"] = "recorded: %s (csrc sha256 %s)" % (tname, csrc_sha()[:12])
+                    out["roofline"]["traffic_source"] = "recorded: profiles/%s (csrc sha256 %s)" % (tname, csrc_sha()[:12])
             except Exception:
                 pass
         # the five largest kernel classes of the instrumented warm-up steps (ms per step, rate as a fraction of the class's roofline):
@@ -622,6 +618,19 @@ def csrc_sha() -> str:
         h.update(f.encode())
         h.update(open(os.path.join(d, f), "rb").read())
     return h.hexdigest()
+
+
+def traffic_record(folder, sha):
+    """(name, contents) of the step's traffic record in ``folder`` that was taken with the kernel sources ``sha``, whatever it is called;
+    (name of the last one, None) if there are only others, (None, None) if there is none"""
+    import glob
+    paths = sorted(glob.glob(os.path.join(folder, "*_pmc_step_traffic.json")))
+    for path in reversed(paths):
+        with open(path) as f:
+            rec = json.load(f)
+        if rec.get("_meta", {}).get("csrc_sha256") == sha:
+            return os.path.basename(path), rec
+    return (os.path.basename(paths[-1]) if paths else None), None
 
 
 def host_cores() -> int:

@@ -3,7 +3,7 @@
 # not fit one pass; --pmc is never combined with the trace domains gpurun refuses).  Writes gpurun_out/pmc_step/summary.json:
 #   per kernel name and per bench.py kernel CLASS: launches, fetched / written MB per launch (FETCH_SIZE x2: gfx950 counts wide
 #   coalesced reads at one half, guide MI355X_MICROARCH.md "HBM"), and _meta.csrc_sha256 = the sha of the kernel sources the
-#   profile belongs to (bench.py reports `traffic` only while that sha matches).  Copy it to profiles/rNN_pmc_step_traffic.json.
+#   profile belongs to (bench.py reports `traffic` only while that sha matches).  Copy it to profiles/NAME_pmc_step_traffic.json.
 # usage (GPU box): bash tools/pmc_step.sh
 cd /tmp && export TMPDIR=/tmp && cd $GRAFT_REPO_ROOT
 mkdir -p gpurun_out/pmc_step
