@@ -11,8 +11,13 @@
 //
 // As in attention.hip, the first product is formed with the "other" sequence index on the LANE (v_mfma_f32_32x32x16_bf16):
 //   forward / dQ : S^T[key][row] = K . Q^T, row softmax in-lane + one half swap;      dK, dV : S[row][key] = Q . K^T
-// so the accumulator, packed to bf16, is the B operand of the second product.  Rounding to bf16 of P and dS is the only rounding
-// between the inputs and the f32 accumulators; softmax sums, statistics and norms stay f32.
+// so the accumulator, packed to bf16, is the B operand of the second product.  Softmax sums, statistics, lambda and norms stay in f32.
+// Rounded to bf16 between the inputs and the results, each by half a step at most (2^-8 of the value; 1.7e-3 in the 2-norm):
+//   P (forward), A = P1 - lam P2 and dS (gradient), dO behind the norm: operands of matrix products, which take bf16 -- two terms each would
+//   be twice the products;
+//   the saved o and o2, from which the gradient forms the norm and dO . O1, dO . O2 again: f32 ones would be 512 bytes more a
+//   head row to write and as many to read, by the bytes 30 us at 32 x 1568 x 3 heads, and take 0.7e-3, in squares, off dq and dk.
+// 2-norms against 64 bits (32 x 160 x 6 heads): outputs 2.2e-3, dv 3.1e-3, dq and dk 3.6e-3; a rounding of the exact results alone is 1.7e-3.
 #include "common.h"
 #include "../../include/mofo_hip.h"
 #include <algorithm>
@@ -27,7 +32,8 @@ constexpr float EMPTY_LSE = 1.0e30f;    // log-sum of a row that sees nothing: e
 // Forward: a row's reference maximum is kept until a score lies more than this many log2 units above it.  The row's outputs are divided
 // by the sum of the ROUNDED terms, so that the rounding of a term that dominates its row cancels; the reference follows a term that is
 // far above it, which is then 1 and not rounded at all.  (Gradients are formed from differences G - d in which such a term cancels: with
-// the sum of the unrounded terms and a reference kept up to 2^20, dq of 160 and 50 tokens was 6e-3 and 1e-2 off; this way 3e-3.)
+// the sum of the unrounded terms and a reference kept up to 2^20, dq of 160 and 50 tokens was 6e-3 and 1e-2 off.  This way 3.6e-3 for 160
+// tokens; kept up to 2^2.5 it is 3.0e-3, and the training step of 32 x 1568 x 3 heads 3 % longer, with the maximum always followed 2.7e-3.)
 constexpr float KEEP_REF = 5.f;
 // Exponents are c s - c (reference) in one fused step while the references of a wave's rows lie below this many log2 units: the rounding of
 // c (reference), 2^-15, is the same for all of a row's terms of one reference, and that small against those of another.  Once one lies
@@ -321,9 +327,9 @@ __device__ __forceinline__ float frag_sum(bf16x8 f, float acc) {
 // 24 matrix instructions (768 cycles of the matrix unit) and about 150 others, 32 of them exponentials at twice the time (740 cycles), stand
 // against the 1850 cycles a tile that a SIMD takes: matrix unit 39 % and vector unit 45 % busy, LDS 15 %, two waves a SIMD (the
 // registers allow no third) whose phases meet too often, at the 1.9 to 2.1 GHz that the card holds.  16 clips x 6 heads x 1568 tokens
-// 209 us, 578 TFLOP/s; one clip of 12544 750 us, 645 TFLOP/s; one clip of 1568 29 us.  (FLOP as the formula has them, 512 a row and key; each
+// 211 us, 573 TFLOP/s; one clip of 12544 752 to 762 us, 640 TFLOP/s; one clip of 1568 29 us.  (FLOP as the formula has them, 512 a row and key; each
 // map's own second product makes 768 of it, since neither sum is known before the last key: 16 x 6 x 2048, whose blocks fill three rounds,
-// runs at 680, that is 1020 TFLOP/s of matrix work, 85 % of a large library product's rate.)  At 1568, without exponentials it is 7 % faster,
+// runs at 620 to 664, that is up to 996 TFLOP/s of matrix work, 83 % of a large library product's rate.)  At 1568, without exponentials it is 7 % faster,
 // without the second products 23 %, without loads 10 %.  Tried without gain: blocks of eight waves whose two halves do products and
 // softmax in opposite phases, a barrier between; the two maps' first products in turn; the next tile's first fragments ahead of the
 // barrier; fences that interleave exponentials and products.  One wave a SIMD, a tile ahead, needs copies between the two halves of the
@@ -657,7 +663,7 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 
 // joins the ranges of a row: one wave a row, lanes 0..31 the first map's 128 columns, lanes 32..63 the second's; the ranges' weights are
 // exp2(c (reference - largest reference) + log2-sum) over their sum, lane s of a half holding ranges s and s + 32.  A chain of latencies: the
-// first sixteen ranges' loads go out before anything is waited for (one token against 16 caches of 8192, 16 ranges: 5.5 us, 6.5 in rounds of eight behind the weights).
+// first sixteen ranges' loads go out before anything is waited for (one token against 16 caches of 8192, 16 ranges: 5.7 us, 6.5 in rounds of eight behind the weights).
 __global__ __launch_bounds__(256) void diff_join_kernel(DiffArgs a, FwdOut f, int nsplit) {
     constexpr int AT_ONCE = 16;
     const int lane = threadIdx.x & 63, m = lane >> 5, sl = lane & 31, d = sl * 4;
