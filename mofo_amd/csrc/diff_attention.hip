@@ -35,9 +35,9 @@ constexpr float EMPTY_LSE = 1.0e30f;    // log-sum of a row that sees nothing: e
 // the sum of the unrounded terms and a reference kept up to 2^20, dq of 160 and 50 tokens was 6e-3 and 1e-2 off.  This way 3.6e-3 for 160
 // tokens; kept up to 2^2.5 it is 3.0e-3, and the training step of 32 x 1568 x 3 heads 3 % longer, with the maximum always followed 2.7e-3.)
 constexpr float KEEP_REF = 5.f;
-// Exponents are c s - c (reference) in one fused step while the references of a wave's rows lie below this many log2 units: the rounding of
-// c (reference), 2^-15, is the same for all of a row's terms of one reference, and that small against those of another.  Once one lies
-// beyond, the wave forms the differences first, exactly, at one more instruction a term, and takes every tile's maximum for reference.
+// Exponents are c s - c (reference) in one fused step while a row's reference lies below this many log2 units: the rounding of c (reference),
+// 2^-15, is the same for all of a row's terms of one reference, and that small against those of another.  Beyond it the reference is taken
+// off the row's scores first, exactly; a wave with such a row looks at every tile's references.  A row's numbers are its own either way.
 constexpr float FAR_REF = 1024.f;
 
 struct DiffArgs {
@@ -89,6 +89,7 @@ __device__ __forceinline__ float head_lambda(const DiffArgs& a, int h, int lane,
     return e1 - e2 + a.lam_init;
 }
 
+__device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
 
 // A lane's byte offsets into a [32][64] half tile, LDS base included (the base a multiple of 128): k step ks of the rows is row ^ 32 ks, columns
@@ -402,8 +403,9 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
     }
 
     const FragOff fo = frag_off(lds0 + ring, lane);
-    float keep = KEEP_REF / a.c;                          // in score units; far references: -inf, every tile takes the branch below
-    float cm = a.c;                                       // what the reference is scaled with in an exponent: 0 where the difference is formed first
+    const float keep = uniform(KEEP_REF / a.c);           // in score units
+    float look = keep;                                    // -inf once a row's reference is far: every tile takes the branch below
+    auto is_far = [&](float x) { return x > -__builtin_inff() && fabsf(x * a.c) > FAR_REF; };
     for (int t = 0; t < nkt; ++t) {
         if constexpr (KEYS4) {
             landed_own();
@@ -448,11 +450,12 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
             for (int r = 1; r < 16; ++r) tm[m] = fmaxf(tm[m], s[m][r]);
             if (m == 0) __builtin_amdgcn_sched_barrier(0);      // the first map's maximum while the second's scores are on their way
         }
-        if (__any(tm[0] > mx[0] + keep || tm[1] > mx[1] + keep)) {            // the first tile (reference -inf) too
+        float taken[2] = {0.f, 0.f};                      // what the scores are already less by
+        if (__any(!(tm[0] <= mx[0] + look) || !(tm[1] <= mx[1] + look))) {    // the first tile (reference -inf) too
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 const float x = fmaxf(tm[m], __shfl_xor(tm[m], 32, 64));
-                const bool up = x > mx[m] + (cm == 0.f ? 0.f : keep);
+                const bool up = x > mx[m] + keep;
                 const float alpha = up ? fast_exp2((mx[m] - x) * a.c) : 1.f;
                 mx[m] = up ? x : mx[m];
                 l[m] *= alpha;
@@ -462,18 +465,19 @@ __global__ __launch_bounds__(256, 2) void diff_fwd_kernel(DiffArgs a, FwdOut f, 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[m][dt][r] *= alpha;
             }
-            auto is_far = [&](float x) { return x > -__builtin_inff() && fabsf(x * a.c) > FAR_REF; };
-            if (cm == 0.f || __ballot(is_far(mx[0]) || is_far(mx[1])) != 0) {
-                cm = 0.f;
-                keep = -__builtin_inff();
+            const bool far[2] = {is_far(mx[0]), is_far(mx[1])};
+            if (__ballot(far[0] || far[1]) != 0) {
+                look = -__builtin_inff();
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
+                for (int m = 0; m < 2; ++m) {
+                    taken[m] = far[m] ? mx[m] : 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[m][r] -= mx[m];
+                    for (int r = 0; r < 16; ++r) s[m][r] -= taken[m];
+                }
             }
         }
         // two halves of 16 keys: the second half's exponentials stand beside the first half's products
-        const float nmc[2] = {-mx[0] * cm, -mx[1] * cm};
+        const float nmc[2] = {(taken[0] - mx[0]) * a.c, (taken[1] - mx[1]) * a.c};
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
             if (KEYS4 && s2 == 1) {

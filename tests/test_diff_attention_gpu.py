@@ -791,3 +791,38 @@ def test_diff_attention_same_bits_at_any_scale(dev, B, Nq, Nk, H, Hkv, causal, p
     for n in want:
         scaled = {"dq": 1 / half, "dk": 1 / rest}.get(n, 1.0)
         assert torch.equal(got[n], want[n] * scaled), n
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_far_and_bad_rows_leave_their_neighbours_alone(dev, B, Nq, Nk, H, Hkv, causal):
+    """one visible query row with scores of 2^40, and another whose scores are NaN: no bit of any other row moves, with near and with far scores of
+    the others"""
+    for offset in (0.0, 2.0 ** 16):
+        q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, offset or 1.0)
+        args = lambda t: (t, k, v, B, H, Hkv, 0.125, lam, 0.4, None, 1.0, None, causal)  # noqa: E731
+        want = _call(*args(q))["out"]
+        q2, far, bad = q.clone(), Nq * B - 1, Nq * B - (2 if Nq * B > 1 else 1)
+        q2[far, :128] *= 2.0 ** 40
+        q2[bad, (H - 1) * 128 + 70] = math.nan
+        got = _call(*args(q2))["out"]
+        assert bool(torch.isfinite(got[far, :128].float()).all()) and bool(torch.isnan(got[bad, (H - 1) * 128:]).all())
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[far, :128] = same[bad, (H - 1) * 128:] = False
+        assert torch.equal(got[same], want[same])
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hkv,causal", FAR)
+def test_diff_attention_far_scores_and_rows_that_see_nothing(dev, norm, B, Nq, Nk, H, Hkv, causal):
+    """lengths from none to all with scores far from zero: rows that see nothing give zeros, whatever they hold"""
+    q, k, v, lam = _far_scores(dev, B, Nq, Nk, H, Hkv, 2.0 ** 16)
+    gamma = _rand((128,), dev, 9, 1.0, F32) if norm else None
+    for lens in ([(b * 37) % (Nk + 1) for b in range(B)], [Nk - (b * 11) % (Nk + 1) for b in range(B)]):
+        kv_len = torch.tensor(lens, dtype=I32, device=dev)
+        args = lambda t: (t, k, v, B, H, Hkv, 0.125, lam, 0.4, gamma, 0.6 if norm else 1.0, kv_len, causal)  # noqa: E731
+        want = _reference(*args(q))
+        got = _call(*args(q))
+        _check(got, want)
+        q2 = q.clone()
+        q2[(_limits(B, Nq, Nk, kv_len, causal, dev) == 0).reshape(-1)] = math.nan
+        assert torch.equal(_call(*args(q2))["out"], got["out"])
